@@ -11,7 +11,8 @@ from ._lib import FusorCudaError, load  # noqa: F401
 
 load()
 
+from ._lib import BF16, F16, F32, I8, U32  # noqa: E402,F401
 from .device import Device  # noqa: E402,F401
 from .tensor import MaskKind, Tensor  # noqa: E402,F401
 from .cache import AttentionMask, KvCache, LlamaCache, MaskCache, PagedKvCache  # noqa: E402,F401
-from .rope import RopeCache, rope  # noqa: E402,F401
+from .rope import RopeCache, axes_of_sections, rope, rope_axes  # noqa: E402,F401

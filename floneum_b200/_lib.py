@@ -13,6 +13,8 @@ from . import build as _build
 
 OK, INVALID_ARGUMENT, SHAPE_MISMATCH, UNSUPPORTED, CUDA_ERROR, NO_DEVICE, TIMEOUT, OUT_OF_PAGES, INTERNAL, NCCL_ERROR = range(10)
 F32, BF16, F16 = 0, 1, 2
+I8 = 3   # pages of a KV cache
+U32 = 4  # positions (host mirror only: they travel as a bare pointer)
 MASK_NONE, MASK_QK, MASK_BATCH_KEY, MASK_CAUSAL, MASK_SLIDING = range(5)
 
 STATUS_NAMES = ["OK", "INVALID_ARGUMENT", "SHAPE_MISMATCH", "UNSUPPORTED", "CUDA_ERROR", "NO_DEVICE", "TIMEOUT",
@@ -28,6 +30,11 @@ class Tensor2(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("shape", c_int64 * 2), ("stride", c_int64 * 2)]
 
 
+class RopePositions(ctypes.Structure):
+    _fields_ = [("ids", c_void_p), ("axis_stride", c_int64), ("batch_stride", c_int64), ("n_axes", c_int32), ("_pad", c_int32),
+                ("axis_of_pair", c_void_p)]
+
+
 class FusorCudaError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[{STATUS_NAMES[code] if 0 <= code < len(STATUS_NAMES) else code}] {message}")
@@ -37,6 +44,7 @@ class FusorCudaError(RuntimeError):
 
 _T4 = POINTER(Tensor4)
 _T2 = POINTER(Tensor2)
+_RP = POINTER(RopePositions)
 
 # name -> (restype, argtypes); every symbol include/fusor_cuda.h declares
 SIGNATURES = {
@@ -62,6 +70,8 @@ SIGNATURES = {
     "fusor_cuda_selftest_wait_limit": (c_int32, [c_void_p]),
     "fusor_cuda_kvcache_create": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                             POINTER(c_void_p)]),
+    "fusor_cuda_kvcache_create_dtype": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                  POINTER(c_void_p)]),
     "fusor_cuda_kvcache_destroy": (c_int32, [c_void_p]),
     "fusor_cuda_kvcache_reset": (c_int32, [c_void_p]),
     "fusor_cuda_kvcache_append": (c_int32, [c_void_p, _T4, _T4]),
@@ -83,6 +93,8 @@ SIGNATURES = {
     "fusor_cuda_attention_out_proj_all_reduce": (c_int32, [c_void_p, c_void_p, _T4, _T4, c_void_p, _T4]),
     "fusor_cuda_rope": (c_int32, [c_void_p, _T4, c_void_p, c_void_p, c_int32, c_int32, c_int32, _T4]),
     "fusor_cuda_kvcache_rope_append": (c_int32, [c_void_p, _T4, _T4, _T4, c_void_p, c_void_p, c_int32, c_int32, c_int32, _T4]),
+    "fusor_cuda_rope_axes": (c_int32, [c_void_p, _T4, c_void_p, c_void_p, c_int32, _RP, c_int32, _T4]),
+    "fusor_cuda_kvcache_rope_axes_append": (c_int32, [c_void_p, _T4, _T4, _T4, c_void_p, c_void_p, c_int32, _RP, c_int32, _T4]),
     "fusor_cuda_kvcache_truncate_front": (c_int32, [c_void_p, c_int32, c_int32]),
     "fusor_cuda_kvcache_drop_front": (c_int32, [c_void_p, c_int32, c_int32]),
     "fusor_cuda_kvcache_seq_len": (c_int32, [c_void_p, c_int32, POINTER(c_int32)]),
@@ -90,6 +102,9 @@ SIGNATURES = {
     "fusor_cuda_kvcache_write_pages": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "fusor_cuda_kvcache_read_pages": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "fusor_cuda_kvcache_pools": (c_int32, [c_void_p, POINTER(c_void_p), POINTER(c_void_p)]),
+    "fusor_cuda_kvcache_write_scales": (c_int32, [c_void_p, c_int32, c_int32, c_void_p]),
+    "fusor_cuda_kvcache_read_scales": (c_int32, [c_void_p, c_int32, c_int32, c_void_p]),
+    "fusor_cuda_kvcache_scales": (c_int32, [c_void_p, POINTER(c_void_p)]),
     "fusor_cuda_kvcache_gather": (c_int32, [c_void_p, _T4, _T4]),
     "fusor_cuda_flash_attention_decode": (c_int32, [c_void_p, c_void_p, _T4, c_float, _T4]),
     "fusor_cuda_flash_attention_decode_partial": (c_int32, [c_void_p, c_void_p, _T4, c_float, c_void_p]),

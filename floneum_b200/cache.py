@@ -3,7 +3,7 @@
 Reference: `AttentionMask` (fusor-ml/fusor/src/cache/attention_mask.rs:10-81), `MaskCache`
 (mask_cache.rs:10-116), `KvCache` (kv_cache.rs:12-68) on `TensorCache` (tensor_cache.rs:9-124).
 The reference keeps dense f32 K/V tensors and copies the whole valid cache on every append;
-here `KvCache` sits on the paged bf16 cache of libfusor_cuda.so and `append` hands back views
+here `KvCache` sits on the paged cache of libfusor_cuda.so (bf16 pages, or 8-bit ones) and `append` hands back views
 that `Tensor.flash_attention` recognises, so a decode step reads the pages in place.
 """
 from __future__ import annotations
@@ -107,17 +107,20 @@ class MaskCache:
 
 # ======================================================================================= paged cache
 class PagedKvCache:
-    """Handle of a `fusor_cuda_kvcache`: bf16 pools [num_pages][Hkv][16][D] + page table + lengths."""
+    """Handle of a `fusor_cuda_kvcache`: pools [num_pages][Hkv][16][D] + page table + lengths.
+
+    dtype BF16, or I8: int8 pools with a scale byte per row, uint8 [num_pages][Hkv][2][16] (K, V).  A row stands for
+    code * 2^(byte - 127), a bf16 number; half the memory and half the bytes of a decode step."""
 
     def __init__(self, device: Device, max_batch: int, num_kv_heads: int, head_dim: int, num_pages: int,
-                 max_pages_per_seq: int, page_tokens: int = PAGE_TOKENS):
+                 max_pages_per_seq: int, page_tokens: int = PAGE_TOKENS, dtype: int = BF16):
         self.device = device
         self.max_batch, self.num_kv_heads, self.head_dim = max_batch, num_kv_heads, head_dim
-        self.num_pages, self.max_pages_per_seq, self.page_tokens = num_pages, max_pages_per_seq, page_tokens
+        self.num_pages, self.max_pages_per_seq, self.page_tokens, self.dtype = num_pages, max_pages_per_seq, page_tokens, dtype
         self._L = _lib.load()
         h = ctypes.c_void_p()
-        _lib.check(self._L.fusor_cuda_kvcache_create(device.handle, max_batch, num_kv_heads, head_dim, page_tokens,
-                                                     num_pages, max_pages_per_seq, ctypes.byref(h)), device.handle)
+        _lib.check(self._L.fusor_cuda_kvcache_create_dtype(device.handle, max_batch, num_kv_heads, head_dim, page_tokens,
+                                                           num_pages, max_pages_per_seq, dtype, ctypes.byref(h)), device.handle)
         self._h = h
 
     def close(self):
@@ -142,14 +145,24 @@ class PagedKvCache:
         self._ck(self._L.fusor_cuda_kvcache_append(self._h, ctypes.byref(ck), ctypes.byref(cv)))
 
     def rope_append(self, q: Tensor, k_new: Tensor, v_new: Tensor, cos: Tensor, sin: Tensor, start_pos: int = -1,
-                    interleaved: bool = False, out_dtype: Optional[int] = None) -> Tensor:
+                    interleaved: bool = False, out_dtype: Optional[int] = None, positions: Optional[Tensor] = None,
+                    axes=None) -> Tensor:
         """RoPE of q and k_new plus the append of (rotated k, v) in one kernel; returns rotated q.
 
-        cos, sin: f32 device tensors [context, D/2].  start_pos < 0: each sequence's own length."""
+        cos, sin: f32 device tensors [context, D/2].  start_pos < 0: each sequence's own length.  `positions` (u32
+        [n_axes, (B,) n]) with `axes` (the axis of each pair) take its place for tokens with several positions."""
+        assert (positions is None) == (axes is None), "positions and axes come together"
         assert tuple(cos.shape()) == tuple(sin.shape()) and cos.shape()[1] == self.head_dim // 2
         assert cos.dtype == F32 and sin.dtype == F32 and cos.is_contiguous() and sin.is_contiguous()
         q_out = Tensor.empty(self.device, q.shape(), q.dtype if out_dtype is None else out_dtype)
         cq, ck, cv, co = q._c4(), k_new._c4(), v_new._c4(), q_out._c4()
+        if positions is not None:
+            from .rope import _positions
+            pos, keep = _positions(positions, axes, q.shape()[0], q.shape()[2], self.head_dim)
+            self._ck(self._L.fusor_cuda_kvcache_rope_axes_append(self._h, ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv),
+                                                                 cos.ptr, sin.ptr, cos.shape()[0], ctypes.byref(pos),
+                                                                 int(bool(interleaved)), ctypes.byref(co)))
+            return q_out
         self._ck(self._L.fusor_cuda_kvcache_rope_append(self._h, ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv),
                                                         cos.ptr, sin.ptr, cos.shape()[0], int(start_pos),
                                                         int(bool(interleaved)), ctypes.byref(co)))
@@ -176,9 +189,10 @@ class PagedKvCache:
                                                            pt.shape[0]))
 
     def write_pages(self, first_page: int, k_bits: np.ndarray, v_bits: np.ndarray):
-        """k_bits, v_bits: uint16 bf16 bit patterns [n_pages, Hkv, page_tokens, D]."""
-        k_bits = np.ascontiguousarray(k_bits, dtype=np.uint16)
-        v_bits = np.ascontiguousarray(v_bits, dtype=np.uint16)
+        """k_bits, v_bits: uint16 bf16 bit patterns [n_pages, Hkv, page_tokens, D]; int8 codes for an 8-bit cache, whose
+        scale bytes go with `write_scales`."""
+        k_bits = np.ascontiguousarray(k_bits, dtype=self._page_type())
+        v_bits = np.ascontiguousarray(v_bits, dtype=self._page_type())
         assert k_bits.shape[1:] == (self.num_kv_heads, self.page_tokens, self.head_dim) and v_bits.shape == k_bits.shape
         self._ck(self._L.fusor_cuda_kvcache_write_pages(self._h, first_page, k_bits.shape[0],
                                                         k_bits.ctypes.data_as(ctypes.c_void_p),
@@ -187,10 +201,31 @@ class PagedKvCache:
 
     def read_pages(self, first_page: int, n_pages: int):
         shape = (n_pages, self.num_kv_heads, self.page_tokens, self.head_dim)
-        k, v = np.empty(shape, np.uint16), np.empty(shape, np.uint16)
+        k, v = np.empty(shape, self._page_type()), np.empty(shape, self._page_type())
         self._ck(self._L.fusor_cuda_kvcache_read_pages(self._h, first_page, n_pages, k.ctypes.data_as(ctypes.c_void_p),
                                                        v.ctypes.data_as(ctypes.c_void_p)))
         return k, v
+
+    def _page_type(self):
+        return np.int8 if self.dtype == _lib.I8 else np.uint16
+
+    def write_scales(self, first_page: int, scales: np.ndarray):
+        """scales: uint8 [n_pages, Hkv, 2, page_tokens] (K, V) of an 8-bit cache."""
+        scales = np.ascontiguousarray(scales, dtype=np.uint8)
+        assert scales.shape[1:] == (self.num_kv_heads, 2, self.page_tokens)
+        self._ck(self._L.fusor_cuda_kvcache_write_scales(self._h, first_page, scales.shape[0], scales.ctypes.data_as(ctypes.c_void_p)))
+        self.device.synchronize()
+
+    def read_scales(self, first_page: int, n_pages: int) -> np.ndarray:
+        scales = np.empty((n_pages, self.num_kv_heads, 2, self.page_tokens), np.uint8)
+        self._ck(self._L.fusor_cuda_kvcache_read_scales(self._h, first_page, n_pages, scales.ctypes.data_as(ctypes.c_void_p)))
+        return scales
+
+    def scales(self) -> int:
+        """Device pointer of an 8-bit cache's scale bytes."""
+        p = ctypes.c_void_p()
+        self._ck(self._L.fusor_cuda_kvcache_scales(self._h, ctypes.byref(p)))
+        return p.value
 
     def pools(self) -> Tuple[int, int]:
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
@@ -283,17 +318,20 @@ class KvCache:
     (models/kalosm-llama/src/raw/cache.rs:26-39).  Past `max_sequence_len` the oldest rows are
     dropped, like TensorCache::append (tensor_cache.rs:55-78)."""
 
-    def __init__(self, concat_dim: int, max_sequence_len: int):
+    def __init__(self, concat_dim: int, max_sequence_len: int, dtype: int = BF16):
+        if dtype not in (BF16, _lib.I8):
+            raise _lib.FusorCudaError(_lib.UNSUPPORTED, f"cache pages are bf16 or 8-bit (dtype {dtype})")
         if concat_dim != 2:
             raise _lib.FusorCudaError(_lib.UNSUPPORTED, "KvCache concatenates along axis 2 of [B, Hkv, S, D] only")
         self.concat_dim = concat_dim
         self.max_sequence_len = max_sequence_len
+        self.dtype = dtype
         self._paged: Optional[PagedKvCache] = None
         self._batch = self._num_kv_heads = self._head_dim = 0
 
     @classmethod
-    def new(cls, concat_dim: int, max_sequence_len: int) -> "KvCache":
-        return cls(concat_dim, max_sequence_len)
+    def new(cls, concat_dim: int, max_sequence_len: int, dtype: int = BF16) -> "KvCache":
+        return cls(concat_dim, max_sequence_len, dtype)
 
     def current_seq_len(self) -> int:
         return self._paged.seq_len(0) if self._paged is not None and self._batch else 0
@@ -316,7 +354,7 @@ class KvCache:
         assert tuple(v.shape()) == (B, Hkv, n, D), "k and v shapes differ"
         if self._paged is None or B > self._paged.max_batch or (self._num_kv_heads, self._head_dim) != (Hkv, D):
             pages_per_seq = (self.max_sequence_len + PAGE_TOKENS - 1) // PAGE_TOKENS + 1
-            self._paged = PagedKvCache(device, B, Hkv, D, B * pages_per_seq, pages_per_seq)
+            self._paged = PagedKvCache(device, B, Hkv, D, B * pages_per_seq, pages_per_seq, dtype=self.dtype)
             self._num_kv_heads, self._head_dim = Hkv, D
         mx = self.max_sequence_len
         skip = 0
@@ -336,41 +374,48 @@ class KvCache:
         self._batch = k.shape()[0]
         return CachedKv(self, "k"), CachedKv(self, "v")
 
-    def _append_rotated(self, rope_cache, q: Tensor, k: Tensor, v: Tensor, start_pos: int, interleaved: bool, out_dtype):
+    def _append_rotated(self, rope_cache, q: Tensor, k: Tensor, v: Tensor, start_pos: int, interleaved: bool, out_dtype,
+                        positions: Optional[Tensor] = None, axes=None):
         """`RopeCache.forward(q, k, start_pos)` then `append(k, v)` in one launch (see RopeCache.forward_append)."""
         if start_pos < 0:
             start_pos = self.current_seq_len()
         n = k.shape()[2]
         k2, v2, skip = self._make_room(q.device, k, v)
         if skip:  # the rows that do not survive still rotate q; do that with the plain op and append the rest
-            from .rope import rope
-            q_rot = rope(q, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype)
+            from .rope import rope, rope_axes
+            if positions is not None:
+                q_rot = rope_axes(q, rope_cache.cos, rope_cache.sin, positions, axes, interleaved, out_dtype)
+                ps = positions.shape()
+                positions = Tensor(q.device, positions.ptr + skip * positions.strides[-1] * 4, ps[:-1] + (n - skip,), positions.dtype,
+                                   positions.strides, owner=positions)
+            else:
+                q_rot = rope(q, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype)
             dummy = Tensor(q.device, q.ptr + skip * q.strides[2] * (4 if q.dtype == F32 else 2),
                            (q.shape()[0], q.shape()[1], n - skip, q.shape()[3]), q.dtype, q.strides, owner=q)
-            self._paged.rope_append(dummy, k2, v2, rope_cache.cos, rope_cache.sin, start_pos + skip, interleaved, out_dtype)
+            self._paged.rope_append(dummy, k2, v2, rope_cache.cos, rope_cache.sin, start_pos + skip, interleaved, out_dtype, positions, axes)
         else:
-            q_rot = self._paged.rope_append(q, k2, v2, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype)
+            q_rot = self._paged.rope_append(q, k2, v2, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype, positions, axes)
         self._batch = k.shape()[0]
         return q_rot, CachedKv(self, "k"), CachedKv(self, "v")
 
     # ------------------------------------------------------------------ session export / import
     def export_session(self) -> dict:
-        """The cache as host arrays: {"k", "v": f32 [B, Hkv, len, D], "max_sequence_len"} (what the reference's session
-        save would hold, models/kalosm-llama/src/session.rs:51-69, where it is stubbed out).  Values are the bf16-rounded
-        rows the pages hold; an empty cache exports zero-length arrays."""
+        """The cache as host arrays: {"k", "v": f32 [B, Hkv, len, D], "max_sequence_len", "dtype" of the pages} (what the reference's session
+        save would hold, models/kalosm-llama/src/session.rs:51-69, where it is stubbed out).  Values are what the rows of the
+        pages stand for; an empty cache exports zero-length arrays."""
         n = self.current_seq_len()
         if n == 0:
             z = np.zeros((self._batch, self._num_kv_heads, 0, self._head_dim), np.float32)
-            return {"k": z, "v": z.copy(), "max_sequence_len": self.max_sequence_len}
+            return {"k": z, "v": z.copy(), "max_sequence_len": self.max_sequence_len, "dtype": self.dtype}
         for b in range(self._batch):  # the rows where an import will put them, so that both caches decode to the same bits
             self._paged.truncate_front(b, n)
         k, v = self._dense(F32)
-        return {"k": k.as_slice(), "v": v.as_slice(), "max_sequence_len": self.max_sequence_len}
+        return {"k": k.as_slice(), "v": v.as_slice(), "max_sequence_len": self.max_sequence_len, "dtype": self.dtype}
 
     @classmethod
     def import_session(cls, device: Device, session: dict) -> "KvCache":
         """Rebuilds a cache from `export_session`'s dictionary (dense rows go back into pages through `append`)."""
-        cache = cls(2, int(session["max_sequence_len"]))
+        cache = cls(2, int(session["max_sequence_len"]), int(session.get("dtype", BF16)))
         k, v = np.asarray(session["k"], np.float32), np.asarray(session["v"], np.float32)
         assert k.shape == v.shape and k.ndim == 4, "session k and v must be [B, Hkv, len, D] arrays of one shape"
         if k.shape[2] > 0:
@@ -406,11 +451,11 @@ class LlamaCache:
     CONCAT_DIMENSION = 2
 
     def __init__(self, n_layer: int, context_length: int, sliding_window_type: Optional[int] = None,
-                 sliding_window_size: Optional[int] = None):
+                 sliding_window_size: Optional[int] = None, dtype: int = BF16):
         self.start_time = 0
         self.tokens: list = []
         self.blocks = [KvCache(self.CONCAT_DIMENSION, self.layer_max_seq_len(i, context_length, sliding_window_type,
-                                                                             sliding_window_size))
+                                                                             sliding_window_size), dtype)
                        for i in range(n_layer)]
 
     new = classmethod(lambda cls, *a, **kw: cls(*a, **kw))

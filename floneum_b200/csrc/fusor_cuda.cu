@@ -25,6 +25,8 @@
 #include "../../include/fusor_cuda.h"
 #include "attn_mma16.cuh"
 #include "attn_mma32.cuh"
+#include "cache8.cuh"
+#include "decode8.cuh"
 #include "decode_splitkv.cuh"
 #include "general_attention.cuh"
 #include "prefill_sm100.cuh"
@@ -461,6 +463,8 @@ static int32_t check_device_error(fusor_cuda_ctx* ctx) {
             return fail(ctx, FUSOR_CUDA_TIMEOUT, "a bounded device-side wait ran out at wait site %d (kernel unwound, result invalid)", h >> 8);
         if (h == kErrBadPage)
             return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "page table holds a page index outside the pool");
+        if (h == kErrBadPosition)
+            return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "a rope position is outside the cos/sin tables (row 0 was read instead)");
         return fail(ctx, FUSOR_CUDA_INTERNAL, "device error word = %d", h);
     }
     return FUSOR_CUDA_OK;
@@ -1093,8 +1097,11 @@ extern "C" int32_t fusor_cuda_flash_attention_host(fusor_cuda_ctx* ctx, const fu
 struct fusor_cuda_kvcache {
     fusor_cuda_ctx* ctx = nullptr;
     int max_batch = 0, Hkv = 0, D = 0, PT = 0, num_pages = 0, max_pages = 0;
-    __nv_bfloat16* k_pages = nullptr;
+    __nv_bfloat16* k_pages = nullptr;  // bf16 pages, or
     __nv_bfloat16* v_pages = nullptr;
+    int8_t* k_codes = nullptr;         // 8-bit pages [num_pages][Hkv][16][D]
+    int8_t* v_codes = nullptr;
+    uint8_t* scales = nullptr;         // with those [num_pages][Hkv][2][16] (see cache8.cuh)
     // one device block [end_before: max_batch][end: max_batch][front: max_batch][page_table: max_batch * max_pages], so that an append
     // brings its tables over in a single copy from a host staging vector of the same layout (pageable on purpose: the
     // driver sends a small pageable copy inline with the command stream, which measured 7 us faster per append on the
@@ -1118,7 +1125,7 @@ struct fusor_cuda_kvcache {
     float* part_o = nullptr;          // [max_slots][DEC_GP][D]
     float* part_ml = nullptr;         // [max_slots][DEC_GP][2]
     // dense staging for token-granular eviction, grown on demand
-    __nv_bfloat16* shift_buf = nullptr;
+    uint8_t* shift_buf = nullptr;
     size_t shift_bytes = 0;
 };
 
@@ -1126,13 +1133,27 @@ struct fusor_cuda_kvcache {
 static int kv_end(const fusor_cuda_kvcache* c, int b) { return c->h_front[b] + c->h_kv_len[b]; }
 static int pages_of(int rows) { return (rows + DEC_PT - 1) / DEC_PT; }
 
+// pool of K (0) or V (1), and the bytes of a page in it
+static uint8_t* kv_pool(const fusor_cuda_kvcache* c, int which) {
+    return c->k_codes ? reinterpret_cast<uint8_t*>(which ? c->v_codes : c->k_codes) : reinterpret_cast<uint8_t*>(which ? c->v_pages : c->k_pages);
+}
+static size_t kv_page_bytes(const fusor_cuda_kvcache* c) { return (size_t)c->Hkv * DEC_PT * c->D * (c->k_codes ? 1 : 2); }
+
 static int32_t kv_fail(fusor_cuda_kvcache* c, int32_t code, const char* msg) { return fail(c ? c->ctx : nullptr, code, "%s", msg); }
 
 extern "C" int32_t fusor_cuda_kvcache_create(fusor_cuda_ctx* ctx, int32_t max_batch, int32_t num_kv_heads, int32_t head_dim,
                                              int32_t page_tokens, int32_t num_pages, int32_t max_pages_per_seq,
                                              fusor_cuda_kvcache** out) {
+    return fusor_cuda_kvcache_create_dtype(ctx, max_batch, num_kv_heads, head_dim, page_tokens, num_pages, max_pages_per_seq,
+                                           FUSOR_CUDA_BF16, out);
+}
+
+extern "C" int32_t fusor_cuda_kvcache_create_dtype(fusor_cuda_ctx* ctx, int32_t max_batch, int32_t num_kv_heads, int32_t head_dim,
+                                                   int32_t page_tokens, int32_t num_pages, int32_t max_pages_per_seq, int32_t dtype,
+                                                   fusor_cuda_kvcache** out) {
     if (!ctx || !out) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
     *out = nullptr;
+    if (dtype != FUSOR_CUDA_BF16 && dtype != FUSOR_CUDA_I8) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "cache pages are bf16 or 8-bit (dtype %d)", dtype);
     if (max_batch <= 0 || num_kv_heads <= 0 || num_pages <= 0 || max_pages_per_seq <= 0)
         return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "sizes must be positive");
     if (page_tokens != DEC_PT) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "page_tokens must be %d", DEC_PT);
@@ -1143,22 +1164,33 @@ extern "C" int32_t fusor_cuda_kvcache_create(fusor_cuda_ctx* ctx, int32_t max_ba
     fusor_cuda_kvcache* c = new fusor_cuda_kvcache();
     c->ctx = ctx; c->max_batch = max_batch; c->Hkv = num_kv_heads; c->D = head_dim; c->PT = page_tokens;
     c->num_pages = num_pages; c->max_pages = max_pages_per_seq;
-    const size_t pool_bytes = (size_t)num_pages * num_kv_heads * DEC_PT * head_dim * 2;
+    const bool i8 = dtype == FUSOR_CUDA_I8;
+    const size_t rows = (size_t)num_pages * num_kv_heads * DEC_PT, pool_bytes = rows * head_dim * (i8 ? 1 : 2);
+    void *k_pool = nullptr, *v_pool = nullptr;
     c->max_grid = DEC_CTAS * ctx->num_sms;
     c->max_slots = max_batch * num_kv_heads + c->max_grid;
     auto alloc = [&](auto** p, size_t bytes) { return ctx->pool.plain(bytes, reinterpret_cast<void**>(p)); };
-    bool ok = alloc(&c->k_pages, pool_bytes) == cudaSuccess && alloc(&c->v_pages, pool_bytes) == cudaSuccess &&
+    bool ok = alloc(&k_pool, pool_bytes) == cudaSuccess && alloc(&v_pool, pool_bytes) == cudaSuccess &&
+              (!i8 || alloc(&c->scales, rows * 2) == cudaSuccess) &&
               alloc(&c->d_tables, ((size_t)3 * max_batch + (size_t)max_batch * max_pages_per_seq) * 4) == cudaSuccess &&
               alloc(&c->part_o, (size_t)c->max_slots * DEC_GP * head_dim * 4) == cudaSuccess &&
               alloc(&c->part_ml, (size_t)c->max_slots * DEC_GP * 2 * 4) == cudaSuccess;
+    if (i8) {
+        c->k_codes = static_cast<int8_t*>(k_pool);
+        c->v_codes = static_cast<int8_t*>(v_pool);
+    } else {
+        c->k_pages = static_cast<__nv_bfloat16*>(k_pool);
+        c->v_pages = static_cast<__nv_bfloat16*>(v_pool);
+    }
     if (ok) {
         c->d_end_before = c->d_tables;
         c->d_end = c->d_tables + max_batch;
         c->d_front = c->d_tables + 2 * max_batch;
         c->d_page_table = c->d_tables + 3 * max_batch;
     }
-    if (ok) ok = cudaMemsetAsync(c->k_pages, 0, pool_bytes, ctx->stream) == cudaSuccess &&
-                 cudaMemsetAsync(c->v_pages, 0, pool_bytes, ctx->stream) == cudaSuccess &&
+    if (ok) ok = cudaMemsetAsync(k_pool, 0, pool_bytes, ctx->stream) == cudaSuccess &&
+                 cudaMemsetAsync(v_pool, 0, pool_bytes, ctx->stream) == cudaSuccess &&
+                 (!i8 || cudaMemsetAsync(c->scales, 1, rows * 2, ctx->stream) == cudaSuccess) &&  // the byte of a row of zeros
                  cudaMemsetAsync(c->d_page_table, 0, (size_t)max_batch * max_pages_per_seq * 4, ctx->stream) == cudaSuccess &&
                  cudaMemsetAsync(c->d_end, 0, (size_t)2 * max_batch * 4, ctx->stream) == cudaSuccess;  // ends and fronts
     if (!ok) {
@@ -1174,7 +1206,7 @@ extern "C" int32_t fusor_cuda_kvcache_create(fusor_cuda_ctx* ctx, int32_t max_ba
     for (int i = 0; i < num_pages; ++i) c->free_list[i] = num_pages - 1 - i;  // pop_back hands out page 0 first
     // tensor maps over the pools, {64 columns, num_pages*Hkv*16 rows, D/64 halves}: one copy brings a whole (page, head) tile,
     // half after half, 128-byte swizzle
-    for (int which = 0; which < 2; ++which) {
+    for (int which = 0; which < 2 && !i8; ++which) {
         cuuint64_t dims[3] = {64, (cuuint64_t)num_pages * num_kv_heads * DEC_PT, (cuuint64_t)head_dim / 64};
         cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, 128};
         cuuint32_t box[3] = {64, DEC_PT, (cuuint32_t)head_dim / 64};
@@ -1196,7 +1228,7 @@ extern "C" int32_t fusor_cuda_kvcache_destroy(fusor_cuda_kvcache* c) {
     if (!c) return FUSOR_CUDA_OK;
     DeviceGuard g(c->ctx->device);
     cudaStreamSynchronize(c->ctx->stream);
-    void* ptrs[] = {c->k_pages, c->v_pages, c->d_tables, c->part_o, c->part_ml, c->shift_buf};
+    void* ptrs[] = {c->k_pages, c->v_pages, c->k_codes, c->v_codes, c->scales, c->d_tables, c->part_o, c->part_ml, c->shift_buf};
     for (void* p : ptrs)
         if (p) cudaFree(p);
 
@@ -1300,10 +1332,39 @@ static int32_t kv_reserve(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new
     return FUSOR_CUDA_OK;
 }
 
+// Rows through place_rows_kernel: rotated (where P has tables), to either cache (where P has pages).
+static int32_t place_launch(fusor_cuda_ctx* ctx, const PlaceParams& P) {
+    const long long rows = (long long)P.B * P.n * (P.Hq + (P.pages ? 2 * P.Hkv : 0));
+    const int blocks = (int)std::max<long long>(1, std::min<long long>((rows + 7) / 8, (long long)ctx->num_sms * 16));
+    place_rows_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+    return launch_check(ctx, "place_rows_kernel");
+}
+// The same with k and v of an append, whose pages are reserved here.  The rest of P has been filled in.
+static int32_t place_append(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new, const fusor_cuda_tensor4* v_new, PlaceParams& P) {
+    fusor_cuda_ctx* ctx = c->ctx;
+    TRY(kv_reserve(c, k_new, v_new, &P.lens));
+    DeviceGuard g(ctx->device);
+    P.k_new = k_new->data; P.v_new = v_new->data; P.k_dtype = k_new->dtype; P.v_dtype = v_new->dtype;
+    for (int i = 0; i < 3; ++i) { P.ks[i] = k_new->stride[i]; P.vs[i] = v_new->stride[i]; }
+    P.pages = c->k_codes ? 2 : 1;
+    P.k_pages = c->k_codes ? (void*)c->k_codes : (void*)c->k_pages;
+    P.v_pages = c->k_codes ? (void*)c->v_codes : (void*)c->v_pages;
+    P.scales = c->scales; P.page_table = c->d_page_table;
+    P.max_pages = c->max_pages; P.Hkv = c->Hkv;
+    P.B = (int)k_new->shape[0]; P.n = (int)k_new->shape[2]; P.D = c->D; P.err = ctx->d_err;
+    const int32_t rc = place_launch(ctx, P);
+    if (rc != FUSOR_CUDA_OK) c->lens_dirty = true;  // the lengths did not go with it
+    return rc;
+}
+
 extern "C" int32_t fusor_cuda_kvcache_append(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new,
                                              const fusor_cuda_tensor4* v_new) {
     if (!c || !k_new || !v_new || !k_new->data || !v_new->data) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
     fusor_cuda_ctx* ctx = c->ctx;
+    if (c->k_codes) {
+        PlaceParams P{};
+        return place_append(c, k_new, v_new, P);
+    }
     AppendParams P;
     TRY(kv_reserve(c, k_new, v_new, &P.lens));
     DeviceGuard g(ctx->device);
@@ -1383,6 +1444,42 @@ static int32_t rope_launch(fusor_cuda_ctx* ctx, const RopeParams& P) {
     return launch_check(ctx, "rope_append_kernel");
 }
 
+static void place_q(PlaceParams& P, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* q_out, const float* cos_t, const float* sin_t,
+                    int32_t context_length, int32_t interleaved) {
+    P.q = q->data; P.q_out = q_out->data; P.q_dtype = q->dtype; P.qo_dtype = q_out->dtype; P.Hq = (int)q->shape[1];
+    for (int i = 0; i < 3; ++i) { P.qs[i] = q->stride[i]; P.qos[i] = q_out->stride[i]; }
+    P.cos_t = cos_t; P.sin_t = sin_t; P.context = context_length; P.interleaved = interleaved ? 1 : 0;
+}
+
+static int32_t place_positions(fusor_cuda_ctx* ctx, PlaceParams& P, const fusor_cuda_rope_positions* pos, int64_t head_dim) {
+    if (!pos || !pos->ids || !pos->axis_of_pair) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "null positions");
+    const int half = (int)(head_dim / 2);
+    if (half > (int)sizeof P.axis) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "rope with several axes covers head_dim up to %d", 2 * (int)sizeof P.axis);
+    if (pos->n_axes <= 0) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "n_axes must be positive");
+    if (pos->axis_stride < 0 || pos->batch_stride < 0) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "position strides must not be negative");
+    if (reinterpret_cast<uintptr_t>(pos->ids) % 4) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "positions must be 4-byte aligned");
+    for (int i = 0; i < half; ++i) {
+        if (pos->axis_of_pair[i] >= pos->n_axes)
+            return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "axis_of_pair[%d] = %d, there are %d axes", i, pos->axis_of_pair[i], pos->n_axes);
+        P.axis[i] = pos->axis_of_pair[i];
+    }
+    P.pos = pos->ids; P.pos_axis = pos->axis_stride; P.pos_b = pos->batch_stride; P.err = ctx->d_err;
+    return FUSOR_CUDA_OK;
+}
+
+extern "C" int32_t fusor_cuda_rope_axes(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* x, const float* cos_t, const float* sin_t,
+                                        int32_t context_length, const fusor_cuda_rope_positions* positions, int32_t interleaved,
+                                        const fusor_cuda_tensor4* out) {
+    if (!ctx) return fail(nullptr, FUSOR_CUDA_INVALID_ARGUMENT, "ctx is null");
+    TRY(rope_check(ctx, x, out, cos_t, sin_t, context_length, "x"));
+    DeviceGuard g(ctx->device);
+    PlaceParams P{};
+    place_q(P, x, out, cos_t, sin_t, context_length, interleaved);
+    P.B = (int)x->shape[0]; P.n = (int)x->shape[2]; P.D = (int)x->shape[3];
+    TRY(place_positions(ctx, P, positions, x->shape[3]));
+    return place_launch(ctx, P);
+}
+
 extern "C" int32_t fusor_cuda_rope(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* x, const float* cos_t, const float* sin_t,
                                    int32_t context_length, int32_t start_pos, int32_t interleaved,
                                    const fusor_cuda_tensor4* out) {
@@ -1400,17 +1497,25 @@ extern "C" int32_t fusor_cuda_rope(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4
     return rope_launch(ctx, P);
 }
 
-extern "C" int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q,
-                                                  const fusor_cuda_tensor4* k_new, const fusor_cuda_tensor4* v_new,
-                                                  const float* cos_t, const float* sin_t, int32_t context_length,
-                                                  int32_t start_pos, int32_t interleaved, const fusor_cuda_tensor4* q_out) {
-    if (!c || !k_new || !v_new || !k_new->data || !v_new->data) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
+static int32_t rope_append_check(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* q_out, const fusor_cuda_tensor4* k_new,
+                                 const float* cos_t, const float* sin_t, int32_t context_length) {
     fusor_cuda_ctx* ctx = c->ctx;
     TRY(rope_check(ctx, q, q_out, cos_t, sin_t, context_length, "q"));
     const int B = (int)k_new->shape[0], n = (int)k_new->shape[2];
     if (q->shape[0] != B || q->shape[2] != n || q->shape[3] != c->D)
         return fail(ctx, FUSOR_CUDA_SHAPE_MISMATCH, "q is [%lld,%lld,%lld,%lld]; k_new brings batch %d, %d tokens, cache head_dim %d",
                     (long long)q->shape[0], (long long)q->shape[1], (long long)q->shape[2], (long long)q->shape[3], B, n, c->D);
+    return FUSOR_CUDA_OK;
+}
+
+extern "C" int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q,
+                                                  const fusor_cuda_tensor4* k_new, const fusor_cuda_tensor4* v_new,
+                                                  const float* cos_t, const float* sin_t, int32_t context_length,
+                                                  int32_t start_pos, int32_t interleaved, const fusor_cuda_tensor4* q_out) {
+    if (!c || !k_new || !v_new || !k_new->data || !v_new->data) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
+    fusor_cuda_ctx* ctx = c->ctx;
+    TRY(rope_append_check(c, q, q_out, k_new, cos_t, sin_t, context_length));
+    const int B = (int)k_new->shape[0], n = (int)k_new->shape[2];
     // highest table row any sequence reads
     long long last = (long long)start_pos + n;
     if (start_pos < 0) {
@@ -1419,6 +1524,12 @@ extern "C" int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* c, const f
     }
     if (last > context_length)
         return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "positions up to %lld are outside the %d-row cos/sin tables", last, context_length);
+    if (c->k_codes) {
+        PlaceParams P{};
+        place_q(P, q, q_out, cos_t, sin_t, context_length, interleaved);
+        P.start_pos = start_pos < 0 ? -1 : start_pos;
+        return place_append(c, k_new, v_new, P);
+    }
     RopeParams P{};
     TRY(kv_reserve(c, k_new, v_new, &P.lens));
     DeviceGuard g(ctx->device);
@@ -1432,6 +1543,19 @@ extern "C" int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* c, const f
     const int32_t rc = rope_launch(ctx, P);
     if (rc != FUSOR_CUDA_OK) c->lens_dirty = true;  // the lengths did not go with it
     return rc;
+}
+
+extern "C" int32_t fusor_cuda_kvcache_rope_axes_append(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q,
+                                                       const fusor_cuda_tensor4* k_new, const fusor_cuda_tensor4* v_new, const float* cos_t,
+                                                       const float* sin_t, int32_t context_length, const fusor_cuda_rope_positions* positions,
+                                                       int32_t interleaved, const fusor_cuda_tensor4* q_out) {
+    if (!c || !k_new || !v_new || !k_new->data || !v_new->data) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
+    fusor_cuda_ctx* ctx = c->ctx;
+    TRY(rope_append_check(c, q, q_out, k_new, cos_t, sin_t, context_length));
+    PlaceParams P{};
+    place_q(P, q, q_out, cos_t, sin_t, context_length, interleaved);
+    TRY(place_positions(ctx, P, positions, c->D));
+    return place_append(c, k_new, v_new, P);
 }
 
 extern "C" int32_t fusor_cuda_kvcache_seq_len(fusor_cuda_kvcache* c, int32_t b, int32_t* len) {
@@ -1482,9 +1606,9 @@ extern "C" int32_t fusor_cuda_kvcache_write_pages(fusor_cuda_kvcache* c, int32_t
         return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "page range outside the pool");
     fusor_cuda_ctx* ctx = c->ctx;
     DeviceGuard g(ctx->device);
-    const size_t per = (size_t)c->Hkv * DEC_PT * c->D;
-    CUDA_TRY(ctx, cudaMemcpyAsync(c->k_pages + first_page * per, k_host, n_pages * per * 2, cudaMemcpyHostToDevice, ctx->stream));
-    CUDA_TRY(ctx, cudaMemcpyAsync(c->v_pages + first_page * per, v_host, n_pages * per * 2, cudaMemcpyHostToDevice, ctx->stream));
+    const size_t per = kv_page_bytes(c), at = first_page * per;
+    CUDA_TRY(ctx, cudaMemcpyAsync(kv_pool(c, 0) + at, k_host, n_pages * per, cudaMemcpyHostToDevice, ctx->stream));
+    CUDA_TRY(ctx, cudaMemcpyAsync(kv_pool(c, 1) + at, v_host, n_pages * per, cudaMemcpyHostToDevice, ctx->stream));
     return FUSOR_CUDA_OK;
 }
 
@@ -1495,17 +1619,47 @@ extern "C" int32_t fusor_cuda_kvcache_read_pages(fusor_cuda_kvcache* c, int32_t 
         return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "page range outside the pool");
     fusor_cuda_ctx* ctx = c->ctx;
     DeviceGuard g(ctx->device);
-    const size_t per = (size_t)c->Hkv * DEC_PT * c->D;
-    CUDA_TRY(ctx, cudaMemcpyAsync(k_host, c->k_pages + first_page * per, n_pages * per * 2, cudaMemcpyDeviceToHost, ctx->stream));
-    CUDA_TRY(ctx, cudaMemcpyAsync(v_host, c->v_pages + first_page * per, n_pages * per * 2, cudaMemcpyDeviceToHost, ctx->stream));
+    const size_t per = kv_page_bytes(c), at = first_page * per;
+    CUDA_TRY(ctx, cudaMemcpyAsync(k_host, kv_pool(c, 0) + at, n_pages * per, cudaMemcpyDeviceToHost, ctx->stream));
+    CUDA_TRY(ctx, cudaMemcpyAsync(v_host, kv_pool(c, 1) + at, n_pages * per, cudaMemcpyDeviceToHost, ctx->stream));
     CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
+    return FUSOR_CUDA_OK;
+}
+
+// The scale bytes of whole pages of an 8-bit cache, from or to host memory.
+static int32_t kv_copy_scales(fusor_cuda_kvcache* c, int32_t first_page, int32_t n_pages, const void* from_host, void* to_host) {
+    if (!c || (!from_host && !to_host)) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
+    if (!c->scales) return kv_fail(c, FUSOR_CUDA_UNSUPPORTED, "the cache's pages are bf16: they have no scales");
+    if (first_page < 0 || n_pages < 0 || first_page + (long long)n_pages > c->num_pages)
+        return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "page range outside the pool");
+    fusor_cuda_ctx* ctx = c->ctx;
+    DeviceGuard g(ctx->device);
+    const size_t per = (size_t)c->Hkv * 2 * DEC_PT, n = n_pages * per;
+    if (from_host) {
+        CUDA_TRY(ctx, cudaMemcpyAsync(c->scales + first_page * per, from_host, n, cudaMemcpyHostToDevice, ctx->stream));
+        return FUSOR_CUDA_OK;
+    }
+    CUDA_TRY(ctx, cudaMemcpyAsync(to_host, c->scales + first_page * per, n, cudaMemcpyDeviceToHost, ctx->stream));
+    CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
+    return FUSOR_CUDA_OK;
+}
+extern "C" int32_t fusor_cuda_kvcache_write_scales(fusor_cuda_kvcache* c, int32_t first_page, int32_t n_pages, const void* scales_host) {
+    return kv_copy_scales(c, first_page, n_pages, scales_host, nullptr);
+}
+extern "C" int32_t fusor_cuda_kvcache_read_scales(fusor_cuda_kvcache* c, int32_t first_page, int32_t n_pages, void* scales_host) {
+    return kv_copy_scales(c, first_page, n_pages, nullptr, scales_host);
+}
+extern "C" int32_t fusor_cuda_kvcache_scales(fusor_cuda_kvcache* c, void** scales) {
+    if (!c || !scales) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
+    if (!c->scales) return kv_fail(c, FUSOR_CUDA_UNSUPPORTED, "the cache's pages are bf16: they have no scales");
+    *scales = c->scales;
     return FUSOR_CUDA_OK;
 }
 
 extern "C" int32_t fusor_cuda_kvcache_pools(fusor_cuda_kvcache* c, void** k_pages, void** v_pages) {
     if (!c || !k_pages || !v_pages) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
-    *k_pages = c->k_pages;
-    *v_pages = c->v_pages;
+    *k_pages = kv_pool(c, 0);
+    *v_pages = kv_pool(c, 1);
     return FUSOR_CUDA_OK;
 }
 
@@ -1523,12 +1677,22 @@ extern "C" int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* c, const fusor_
     if (k_out->stride[3] != 1 || v_out->stride[3] != 1) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "the head_dim axis must be contiguous");
     DeviceGuard g(ctx->device);
     TRY(kv_sync_tables(c));
+    const long long total = (long long)c->active_B * c->Hkv * longest * c->D;
+    if (c->k_codes) {
+        Gather8Params P;
+        P.k_out = k_out->data; P.v_out = v_out->data; P.k_dtype = k_out->dtype; P.v_dtype = v_out->dtype;
+        for (int i = 0; i < 3; ++i) { P.ks[i] = k_out->stride[i]; P.vs[i] = v_out->stride[i]; }
+        P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
+        P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.D = c->D; P.len = longest; P.B = c->active_B;
+        const int blocks = (int)std::max<long long>(1, std::min<long long>((total + 255) / 256, (long long)ctx->num_sms * 8));
+        kvcache8_gather_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+        return launch_check(ctx, "kvcache8_gather_kernel");
+    }
     GatherParams P;
     P.k_out = k_out->data; P.v_out = v_out->data; P.k_dtype = k_out->dtype; P.v_dtype = v_out->dtype;
     for (int i = 0; i < 3; ++i) { P.ks[i] = k_out->stride[i]; P.vs[i] = v_out->stride[i]; }
     P.k_pages = c->k_pages; P.v_pages = c->v_pages; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
     P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.D = c->D; P.len = longest; P.B = c->active_B;
-    const long long total = (long long)P.B * P.Hkv * P.len * P.D;
     const int blocks = (int)std::min<long long>((total + 255) / 256, (long long)ctx->num_sms * 8);
     kvcache_gather_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
     return launch_check(ctx, "kvcache_gather_kernel");
@@ -1556,7 +1720,7 @@ static int32_t kv_keep_rows(fusor_cuda_kvcache* c, int b, int keep) {
         // token-granular shift: the kept rows go through a dense staging buffer and back into pages 0.. of the same
         // table row, two launches whatever the length (the row on the device is the one from before the eviction)
         const size_t elems = (size_t)c->Hkv * keep * c->D;
-        if (c->shift_bytes < 2 * elems * 2) {
+        if (c->shift_bytes < 2 * elems * 2) {  // (8-bit rows take less)
             CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
             if (c->shift_buf) CUDA_TRY(ctx, cudaFree(c->shift_buf));
             c->shift_buf = nullptr;
@@ -1566,18 +1730,24 @@ static int32_t kv_keep_rows(fusor_cuda_kvcache* c, int b, int keep) {
             c->shift_bytes = want;
         }
         TRY(kv_sync_tables(c));
-        ShiftParams P;
-        P.k_pages = c->k_pages; P.v_pages = c->v_pages; P.row = c->d_page_table + (size_t)b * c->max_pages;
-        P.sk = c->shift_buf; P.sv = c->shift_buf + c->shift_bytes / 4;
-        P.Hkv = c->Hkv; P.D = c->D; P.keep = keep; P.drop = drop;
-        const long long n_vec = (long long)elems / 8;
+        const long long n_vec = (long long)elems / 8;  // 16-byte vectors of one bf16 pool, or of both 8-bit pools
         const int blocks = (int)std::max<long long>(1, std::min<long long>((n_vec + 255) / 256, (long long)ctx->num_sms * 8));
-        P.to_pages = 0;
-        kvcache_shift_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
-        TRY(launch_check(ctx, "kvcache_shift_kernel"));
-        P.to_pages = 1;
-        kvcache_shift_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
-        TRY(launch_check(ctx, "kvcache_shift_kernel"));
+        const int* table_row = c->d_page_table + (size_t)b * c->max_pages;
+        for (int to_pages = 0; to_pages < 2; ++to_pages) {
+            if (c->k_codes) {
+                const Shift8Params P{{c->k_codes, c->v_codes}, c->scales, table_row, reinterpret_cast<int8_t*>(c->shift_buf), c->shift_buf + 2 * elems,
+                                     c->Hkv, c->D, keep, drop, to_pages};
+                kvcache8_shift_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+                TRY(launch_check(ctx, "kvcache8_shift_kernel"));
+                continue;
+            }
+            ShiftParams P;
+            P.k_pages = c->k_pages; P.v_pages = c->v_pages; P.row = table_row;
+            P.sk = reinterpret_cast<__nv_bfloat16*>(c->shift_buf); P.sv = reinterpret_cast<__nv_bfloat16*>(c->shift_buf + c->shift_bytes / 2);
+            P.Hkv = c->Hkv; P.D = c->D; P.keep = keep; P.drop = drop; P.to_pages = to_pages;
+            kvcache_shift_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+            TRY(launch_check(ctx, "kvcache_shift_kernel"));
+        }
         const int new_pages = pages_of(keep);
         for (int p = new_pages; p < pages_of(end); ++p) {
             c->page_used[row[p]] = 0;
@@ -1698,6 +1868,18 @@ static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fus
     }
     DeviceGuard guard(ctx->device);
     TRY(kv_sync_tables(c));
+    if (c->k_codes) {
+        if (mode == 2) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "the exchange decode takes bf16 pages");
+        Decode8Params P{};
+        P.q = q->data; P.q_dtype = q->dtype; P.q_sb = q->stride[0]; P.q_sh = q->stride[1];
+        P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table;
+        P.max_pages = c->max_pages; P.num_pages = c->num_pages; P.end = c->d_end; P.front = c->d_front;
+        P.B = B; P.Hkv = c->Hkv; P.g = g; P.scale_log2 = scale * 1.4426950408889634f; P.err = ctx->d_err;
+        P.res.out = out; P.res.out_dtype = out_dtype; P.res.o_sb = o_sb; P.res.o_sh = o_sh; P.res.Hq = Hq; P.res.mode = mode;
+        if (c->D == 128) decode8_row_kernel<128><<<dim3(Hq, B), 128, 0, ctx->stream>>>(P);
+        else decode8_row_kernel<64><<<dim3(Hq, B), 128, 0, ctx->stream>>>(P);
+        return launch_check(ctx, "decode8_row_kernel");
+    }
     DecodeParams P{};
     P.q = q->data; P.q_dtype = q->dtype; P.q_sb = q->stride[0]; P.q_sh = q->stride[1];
     P.page_table = c->d_page_table; P.max_pages = c->max_pages; P.num_pages = c->num_pages;

@@ -11,7 +11,7 @@ namespace fusor {
 
 // Error word values written by kernels (host maps any non-zero value to FUSOR_CUDA_TIMEOUT
 // or FUSOR_CUDA_INTERNAL).
-enum : int { kErrNone = 0, kErrWaitTimeout = 1, kErrBadPage = 2 };
+enum : int { kErrNone = 0, kErrWaitTimeout = 1, kErrBadPage = 2, kErrBadPosition = 3 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -20,8 +20,8 @@ import numpy as np
 from . import _lib
 from .device import Device
 
-F32, BF16, F16 = _lib.F32, _lib.BF16, _lib.F16
-_ITEMSIZE = {F32: 4, BF16: 2, F16: 2}
+F32, BF16, F16, U32 = _lib.F32, _lib.BF16, _lib.F16, _lib.U32
+_ITEMSIZE = {F32: 4, BF16: 2, F16: 2, U32: 4}
 
 
 class MaskKind(enum.Enum):
@@ -41,13 +41,13 @@ def _from_bf16_bits(b: np.ndarray) -> np.ndarray:
 
 def _host_bits(a: np.ndarray, dtype: int) -> np.ndarray:
     """f32 host values -> the array that is uploaded for `dtype` (f16: numpy's own round-to-nearest-even)."""
-    if dtype == F32:
+    if dtype in (F32, U32):
         return a
     return _to_bf16_bits(a) if dtype == BF16 else np.ascontiguousarray(a.astype(np.float16)).view(np.uint16)
 
 
 class Tensor:
-    """A strided view of device memory: shape, element strides, dtype (f32, bf16 or f16)."""
+    """A strided view of device memory: shape, element strides, dtype (f32, bf16 or f16; u32 for positions)."""
 
     def __init__(self, device: Device, ptr: int, shape: Sequence[int], dtype: int = F32,
                  strides: Optional[Sequence[int]] = None, owner=None, owns: bool = False):
@@ -75,8 +75,8 @@ class Tensor:
 
     @classmethod
     def from_slice(cls, device: Device, shape: Sequence[int], data, dtype: int = F32) -> "Tensor":
-        """Upload host data (any array-like of floats) as a contiguous tensor of `shape`."""
-        a = np.ascontiguousarray(np.asarray(data, dtype=np.float32).reshape(shape))
+        """Upload host data (any array-like of floats, or of whole numbers for u32) as a contiguous tensor of `shape`."""
+        a = np.ascontiguousarray(np.asarray(data, dtype=np.uint32 if dtype == U32 else np.float32).reshape(shape))
         host = _host_bits(a, dtype)
         t = cls.empty(device, shape, dtype)
         L = _lib.load()
@@ -89,9 +89,9 @@ class Tensor:
 
     @classmethod
     def from_torch(cls, device: Device, t) -> "Tensor":
-        """Borrow a CUDA torch tensor (float32, bfloat16 or float16) without copying."""
+        """Borrow a CUDA torch tensor (float32, bfloat16 or float16; int32 or uint32 for positions) without copying."""
         import torch
-        dt = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}[t.dtype]
+        dt = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: U32, torch.uint32: U32}[t.dtype]
         return cls(device, t.data_ptr(), tuple(t.shape), dt, tuple(t.stride()), owner=t)
 
     @classmethod
@@ -113,14 +113,14 @@ class Tensor:
         return math.prod(self._shape)
 
     def as_slice(self) -> np.ndarray:
-        """Read back as a float32 numpy array indexable like the reference's TensorSlice."""
+        """Read back as a float32 (u32: uint32) numpy array indexable like the reference's TensorSlice."""
         assert self.is_contiguous(), "as_slice needs a contiguous tensor"
-        host = np.empty(self._shape, np.float32 if self.dtype == F32 else np.uint16)
+        host = np.empty(self._shape, {F32: np.float32, U32: np.uint32}.get(self.dtype, np.uint16))
         L = _lib.load()
         _lib.check(L.fusor_cuda_buffer_download(self.device.handle, host.ctypes.data_as(ctypes.c_void_p),
                                                 ctypes.c_void_p(self.ptr), host.nbytes), self.device.handle)
         self.device.synchronize()
-        if self.dtype == F32:
+        if self.dtype in (F32, U32):
             return host
         if self.dtype == F16:
             return host.view(np.float16).astype(np.float32)

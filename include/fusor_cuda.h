@@ -40,6 +40,7 @@ extern "C" {
 #define FUSOR_CUDA_BF16 1
 #define FUSOR_CUDA_F16 2 /* the reference GPU arm is generic over f32 / f16 with f32 accumulation
                             (fusor-ml/core/src/composite/flash_attention.rs:28-38,189) */
+#define FUSOR_CUDA_I8 3  /* pages of a KV cache only (fusor_cuda_kvcache_create_dtype) */
 
 /* ---- mask kinds (enum MaskKind, fusor-ml/fusor/src/composite/flash_attention.rs:10-19) */
 #define FUSOR_CUDA_MASK_NONE 0
@@ -182,6 +183,19 @@ int32_t fusor_cuda_selftest_wait_limit(fusor_cuda_ctx* ctx);
 int32_t fusor_cuda_kvcache_create(fusor_cuda_ctx* ctx, int32_t max_batch, int32_t num_kv_heads, int32_t head_dim,
                                   int32_t page_tokens, int32_t num_pages, int32_t max_pages_per_seq,
                                   fusor_cuda_kvcache** out);
+/* The same with the type of the pages: FUSOR_CUDA_BF16, or FUSOR_CUDA_I8 for half the memory and half the bytes of a decode
+ * step (the reference has no counterpart).  An 8-bit cache holds a row (one token of one kv head, D elements x; rotated, in f32) as
+ * whole numbers of a step of its own, a power of two: with 2^e the smallest, e from -126 to 121, for which max |x| < 127.5 2^e,
+ *   code = x / 2^e rounded to nearest, ties to even, from -127 to 127;   scale byte = e + 127;   the row stands for code 2^e,
+ * which is a bf16 number: gather to any type that has the range, an attention over gathered rows and a decode see the same values, and
+ * appending a gathered row again gives the same codes.  A row with an element that is not finite has the byte 255 and
+ * stands for NaN in all places.
+ *   k_pages, v_pages : int8 [num_pages][Hkv][16][D],   scales : uint8 [num_pages][Hkv][2][16] (K, V)
+ * Every function on a cache takes either kind; write_pages / read_pages move codes (one byte each), the scales go beside
+ * them by the functions below.  A decode takes f32 queries as they are (a bf16 cache rounds them to bf16). */
+int32_t fusor_cuda_kvcache_create_dtype(fusor_cuda_ctx* ctx, int32_t max_batch, int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t page_tokens, int32_t num_pages, int32_t max_pages_per_seq, int32_t dtype,
+                                        fusor_cuda_kvcache** out);
 int32_t fusor_cuda_kvcache_destroy(fusor_cuda_kvcache* cache);
 /* KvCache::reset (kv_cache.rs:42-46): every sequence back to length 0, all pages free. */
 int32_t fusor_cuda_kvcache_reset(fusor_cuda_kvcache* cache);
@@ -207,6 +221,27 @@ int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* cache, const fusor_cu
                                        const fusor_cuda_tensor4* k_new, const fusor_cuda_tensor4* v_new, const float* cos,
                                        const float* sin, int32_t context_length, int32_t start_pos, int32_t interleaved,
                                        const fusor_cuda_tensor4* q_out);
+/* Positions with several axes (time, row and column of an image's or a video's tokens): pair i of the head_dim / 2 pairs of token t
+ * of sequence b takes row ids[axis_of_pair[i] * axis_stride + b * batch_stride + t] of the tables (column i, as ever).
+ *   ids          : device uint32; batch_stride 0 where all sequences have the same
+ *   axis_of_pair : host, head_dim / 2 entries below n_axes; read during the call
+ * A position outside the tables is read as row 0 and reported by the next call that waits for the stream (INVALID_ARGUMENT). */
+typedef struct fusor_cuda_rope_positions {
+    const uint32_t* ids;
+    int64_t axis_stride;
+    int64_t batch_stride;
+    int32_t n_axes;
+    int32_t _pad;
+    const uint8_t* axis_of_pair;
+} fusor_cuda_rope_positions;
+/* fusor_cuda_rope with such positions in place of start_pos + t; head_dim up to 512. */
+int32_t fusor_cuda_rope_axes(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* x, const float* cos, const float* sin, int32_t context_length,
+                             const fusor_cuda_rope_positions* positions, int32_t interleaved, const fusor_cuda_tensor4* out);
+/* fusor_cuda_kvcache_rope_append with such positions: q -> q_out, rotated k and v -> the cache, either kind, in one launch. */
+int32_t fusor_cuda_kvcache_rope_axes_append(fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* k_new,
+                                            const fusor_cuda_tensor4* v_new, const float* cos, const float* sin, int32_t context_length,
+                                            const fusor_cuda_rope_positions* positions, int32_t interleaved,
+                                            const fusor_cuda_tensor4* q_out);
 /* TensorCache eviction (tensor_cache.rs:55-78): keep only the newest `keep` tokens of sequence b.  Whole pages fall
  * off the table row on the host; a drop that is not a multiple of the page size moves the kept rows with two kernel
  * launches (through a staging buffer the cache allocates on first use), whatever the length. */
@@ -230,6 +265,10 @@ int32_t fusor_cuda_kvcache_read_pages(fusor_cuda_kvcache* cache, int32_t first_p
                                       void* v_host);
 /* Device pointers of the pools (for callers that fill pages with their own kernels). */
 int32_t fusor_cuda_kvcache_pools(fusor_cuda_kvcache* cache, void** k_pages, void** v_pages);
+/* The same for the scale bytes of an 8-bit cache, uint8 [n_pages][Hkv][2][16]; UNSUPPORTED on a bf16 cache. */
+int32_t fusor_cuda_kvcache_write_scales(fusor_cuda_kvcache* cache, int32_t first_page, int32_t n_pages, const void* scales_host);
+int32_t fusor_cuda_kvcache_read_scales(fusor_cuda_kvcache* cache, int32_t first_page, int32_t n_pages, void* scales_host);
+int32_t fusor_cuda_kvcache_scales(fusor_cuda_kvcache* cache, void** scales);
 /* Dense export (what KvCache::k()/v() hand back, kv_cache.rs:32-39): k_out, v_out [B,Hkv,len,D] device tensors,
  * len = the longest active sequence; rows past a sequence's length are zero. */
 int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* k_out,

@@ -304,12 +304,14 @@ inline Tensor<4> flash_attention(const Tensor<4>& q, const Tensor<4>& k, const T
     return out;
 }
 
-// KvCache (kv_cache.rs:12-68) on the paged bf16 cache of the library.  concat_dim must be 2, the sequence axis of
+// KvCache (kv_cache.rs:12-68) on the paged cache of the library.  concat_dim must be 2, the sequence axis of
 // [B, Hkv, S, D] (models/kalosm-llama/src/raw/cache.rs:26-39).  Past max_sequence_len the oldest rows are dropped
 // (tensor_cache.rs:55-78).
 class KvCache {
   public:
-    KvCache(size_t concat_dim, size_t max_sequence_len) : max_len_(max_sequence_len) {
+    // cache_dtype: FUSOR_CUDA_BF16, or FUSOR_CUDA_I8 for 8-bit pages (fusor_cuda_kvcache_create_dtype)
+    KvCache(size_t concat_dim, size_t max_sequence_len, int32_t cache_dtype = FUSOR_CUDA_BF16) : max_len_(max_sequence_len), cache_dtype_(cache_dtype) {
+        if (cache_dtype != FUSOR_CUDA_BF16 && cache_dtype != FUSOR_CUDA_I8) throw std::runtime_error("cache pages are bf16 or 8-bit");
         if (concat_dim != 2) throw std::runtime_error("KvCache concatenates along axis 2 of [B, Hkv, S, D] only");
     }
     ~KvCache() {
@@ -336,8 +338,8 @@ class KvCache {
             cache_ = nullptr;
             dev_ = dev;
             const int pages_per_seq = (int)((max_len_ + 15) / 16 + 1);
-            dev->check(fusor_cuda_kvcache_create(dev->raw(), (int32_t)s[0], (int32_t)s[1], (int32_t)s[3], 16, (int32_t)s[0] * pages_per_seq,
-                                                 pages_per_seq, &cache_));
+            dev->check(fusor_cuda_kvcache_create_dtype(dev->raw(), (int32_t)s[0], (int32_t)s[1], (int32_t)s[3], 16, (int32_t)s[0] * pages_per_seq,
+                                                       pages_per_seq, cache_dtype_, &cache_));
             max_batch_ = s[0];
             hkv_ = s[1];
             d_ = s[3];
@@ -387,6 +389,7 @@ class KvCache {
 
   private:
     size_t max_len_;
+    int32_t cache_dtype_;
     DevicePtr dev_;
     fusor_cuda_kvcache* cache_ = nullptr;
     int64_t batch_ = 0, max_batch_ = 0, hkv_ = 0, d_ = 0;
@@ -407,6 +410,7 @@ struct LlamaCacheConfig {
     size_t context_length = 0;
     std::optional<size_t> sliding_window_type;
     std::optional<size_t> sliding_window_size;
+    int32_t cache_dtype = FUSOR_CUDA_BF16;
 };
 
 class LlamaCache {
@@ -415,7 +419,7 @@ class LlamaCache {
     explicit LlamaCache(const LlamaCacheConfig& config) {
         blocks.reserve(config.n_layer);
         for (size_t layer_idx = 0; layer_idx < config.n_layer; ++layer_idx)
-            blocks.push_back(std::make_unique<KvCache>(CONCAT_DIMENSION, layer_max_seq_len(config, layer_idx)));
+            blocks.push_back(std::make_unique<KvCache>(CONCAT_DIMENSION, layer_max_seq_len(config, layer_idx), config.cache_dtype));
     }
     static size_t layer_max_seq_len(const LlamaCacheConfig& config, size_t layer_idx) {
         if (config.sliding_window_type && config.sliding_window_size) {
@@ -458,6 +462,30 @@ inline Tensor<4> rope(const Tensor<4>& x, const Tensor<2>& cos, const Tensor<2>&
     return out;
 }
 
+// The same with a position on each of several axes (see fusor_cuda_rope_positions): pair i of token t takes row
+// ids[axis_of_pair[i]][b][t] of the tables; ids on the device, u32 [n_axes][B or 1][n] packed.
+struct RopeAxes {
+    const uint32_t* ids = nullptr;
+    bool per_sequence = false;  // ids has the batch axis
+    int32_t n_axes = 0;
+    std::vector<uint8_t> axis_of_pair;
+};
+inline Tensor<4> rope_axes(const Tensor<4>& x, const Tensor<2>& cos, const Tensor<2>& sin, const RopeAxes& axes, bool interleaved = false) {
+    if (cos.shape() != sin.shape() || cos.shape()[1] * 2 != x.shape()[3]) throw std::logic_error("rope: cos / sin must be [context, head_dim / 2]");
+    if ((int64_t)axes.axis_of_pair.size() * 2 != x.shape()[3]) throw std::logic_error("rope_axes: axis_of_pair must name the axis of each pair");
+    Tensor<4> out = Tensor<4>::empty(x.device(), x.shape(), x.dtype());
+    const fusor_cuda_tensor4 vx = detail::view4(x), vo = detail::view4(out);
+    fusor_cuda_rope_positions pos{};
+    pos.ids = axes.ids;
+    pos.axis_stride = x.shape()[2] * (axes.per_sequence ? x.shape()[0] : 1);
+    pos.batch_stride = axes.per_sequence ? x.shape()[2] : 0;
+    pos.n_axes = axes.n_axes;
+    pos.axis_of_pair = axes.axis_of_pair.data();
+    x.device()->check(fusor_cuda_rope_axes(x.device()->raw(), &vx, static_cast<const float*>(cos.data()), static_cast<const float*>(sin.data()),
+                                           (int32_t)cos.shape()[0], &pos, interleaved ? 1 : 0, &vo));
+    return out;
+}
+
 class RopeCache {
   public:
     // RopeCache::new (rope.rs:197-219)
@@ -479,6 +507,9 @@ class RopeCache {
     }
     std::pair<Tensor<4>, Tensor<4>> forward_interleaved(const Tensor<4>& q, const Tensor<4>& k, size_t start_pos) const {
         return {rope(q, cos_, sin_, start_pos, true), rope(k, cos_, sin_, start_pos, true)};
+    }
+    std::pair<Tensor<4>, Tensor<4>> forward_axes(const Tensor<4>& q, const Tensor<4>& k, const RopeAxes& axes, bool interleaved = false) const {
+        return {rope_axes(q, cos_, sin_, axes, interleaved), rope_axes(k, cos_, sin_, axes, interleaved)};
     }
     const Tensor<2>& cos() const { return cos_; }
     const Tensor<2>& sin() const { return sin_; }
