@@ -361,6 +361,14 @@ extern "C" int32_t fusor_cuda_ctx_create(int32_t device, void* stream, fusor_cud
         {(const void*)decode_splitkv_kernel<64>, 227 * 1024, "decode_splitkv_kernel<64>"},
         {(const void*)decode_cluster_kernel<128>, (int)DecodeClusterSmem<128>::bytes, "decode_cluster_kernel<128>"},
         {(const void*)decode_cluster_kernel<64>, (int)DecodeClusterSmem<64>::bytes, "decode_cluster_kernel<64>"},
+        {(const void*)decode8_splitkv_kernel<128, 1>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
+        {(const void*)decode8_splitkv_kernel<128, 2>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
+        {(const void*)decode8_splitkv_kernel<64, 1>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
+        {(const void*)decode8_splitkv_kernel<64, 2>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
+        {(const void*)decode8_cluster_kernel<128, 1>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
+        {(const void*)decode8_cluster_kernel<128, 2>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
+        {(const void*)decode8_cluster_kernel<64, 1>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
+        {(const void*)decode8_cluster_kernel<64, 2>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
         {(const void*)attn_mma16_kernel<96, false, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, false, true>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, true, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
@@ -1840,6 +1848,63 @@ static void exchange_merge_params(const fusor_cuda_exchange* ex, PeerMergeParams
 // merge, its partial record and the share of the final merge) is spread over at least this many 8 KB page pairs.
 static constexpr long long kDecodeMinPagesPerCta = 24;
 
+// Merge of the records of every (sequence, kv head) that `grid` CTAs have shared `total` pages of, as the last launch of a decode.
+static int32_t launch_combine(fusor_cuda_kvcache* c, const DecodeOutput& res, int B, int g, int grid, long long total, long long longest,
+                              fusor_cuda_exchange* ex) {
+    fusor_cuda_ctx* ctx = c->ctx;
+    CombineParams C{};
+    C.part_o = c->part_o; C.part_ml = c->part_ml; C.end = c->d_end;
+    C.B = B; C.Hkv = c->Hkv; C.g = g; C.D = c->D; C.grid = grid; C.res = res;
+    // record lanes per block: a kv head of a short sequence has one or two records, a 128 K-token sequence ~74
+    const long long per_head = longest * grid / std::max<long long>(1, total) + 2;
+    const int lanes = per_head <= 4 ? 2 : per_head <= 32 ? 8 : DEC_CL;
+    if (res.mode != 2) {
+        // (the kernel's blocks return at once for heads whose pages all went to one CTA)
+        decode_combine_kernel<<<dim3(res.Hq, B), (c->D / 4) * lanes, 0, ctx->stream>>>(C);
+        return launch_check(ctx, "decode_combine_kernel");
+    }
+    // KV-chunk decode over several GPUs: merge + exchange in one launch
+    CombineExchangeParams X{};
+    X.C = C;
+    exchange_targets(ex, &X.T);
+    exchange_merge_params(ex, &X.M, (int64_t)B * res.Hq, c->D, static_cast<float*>(res.out));
+    const unsigned blocks = (unsigned)std::min<long long>((long long)B * res.Hq, ctx->num_sms);
+    decode_combine_exchange_kernel<<<blocks, (c->D / 4) * lanes, 0, ctx->stream>>>(X);
+    return launch_check(ctx, "decode_combine_exchange_kernel");
+}
+
+// Decode over 8-bit pages, `total` (page, kv head) pairs in all: see decode8.cuh.
+static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, long long total, fusor_cuda_exchange* ex) {
+    fusor_cuda_ctx* ctx = c->ctx;
+    const bool two = P.q_dtype == FUSOR_CUDA_F32;  // query terms
+    long long longest = 0;
+    for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
+    const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;
+    if (P.res.mode != 2 && c->decode_ctas == 0 && heads <= ctx->num_sms && longest >= 1) {
+        int i = 0;
+        while (i < 3 && heads <= ctx->clusters[i + 1]) ++i;
+        const int C = 1 << i;
+        const long long share = (longest + C - 1) / C, share_ns = share * std::max<long long>(126, 161 * heads * C / 128) * unit / 8192;
+        if (share_ns <= 9300 + total * 194 / ctx->num_sms * unit / 8192) {
+            cudaLaunchAttribute attr;
+            const cudaLaunchConfig_t cfg = cluster_config(ctx, (unsigned)(heads * C), (unsigned)C, D8_THREADS,
+                                                          c->D == 128 ? Decode8ClusterSmem<128>::bytes : Decode8ClusterSmem<64>::bytes, &attr);
+            CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, c->D == 128 ? (two ? decode8_cluster_kernel<128, 2> : decode8_cluster_kernel<128, 1>)
+                                                               : (two ? decode8_cluster_kernel<64, 2> : decode8_cluster_kernel<64, 1>), P, C));
+            return launch_check(ctx, "decode8_cluster_kernel");
+        }
+    }
+    const int per_sm = (int)std::max<long long>(1, std::min<long long>(D8_CTAS, total / (32 * ctx->num_sms)));
+    const int grid = (int)std::min<long long>(c->decode_ctas > 0 ? std::min(c->decode_ctas, c->max_grid) : per_sm * ctx->num_sms, total);
+    if (total > 0) {  // (every chunk empty: only the merge kernel runs and writes empty records)
+        const auto run = [&](auto kernel, size_t smem) { kernel<<<grid, D8_THREADS, smem, ctx->stream>>>(P); };
+        if (c->D == 128) run(two ? decode8_splitkv_kernel<128, 2> : decode8_splitkv_kernel<128, 1>, Decode8Smem<128>::bytes);
+        else run(two ? decode8_splitkv_kernel<64, 2> : decode8_splitkv_kernel<64, 1>, Decode8Smem<64>::bytes);
+        TRY(launch_check(ctx, "decode8_splitkv_kernel"));
+    }
+    return launch_combine(c, P.res, P.B, P.g, grid, total, longest, ex);
+}
+
 static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q, float scale, void* out,
                            int out_dtype, long long o_sb, long long o_sh, int mode, fusor_cuda_exchange* ex = nullptr) {
     if (!ctx || !c || !q || !q->data || !out || (mode == 2 && !ex)) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "null argument");
@@ -1869,16 +1934,14 @@ static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fus
     DeviceGuard guard(ctx->device);
     TRY(kv_sync_tables(c));
     if (c->k_codes) {
-        if (mode == 2) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "the exchange decode takes bf16 pages");
         Decode8Params P{};
         P.q = q->data; P.q_dtype = q->dtype; P.q_sb = q->stride[0]; P.q_sh = q->stride[1];
         P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table;
         P.max_pages = c->max_pages; P.num_pages = c->num_pages; P.end = c->d_end; P.front = c->d_front;
         P.B = B; P.Hkv = c->Hkv; P.g = g; P.scale_log2 = scale * 1.4426950408889634f; P.err = ctx->d_err;
+        P.part_o = c->part_o; P.part_ml = c->part_ml;
         P.res.out = out; P.res.out_dtype = out_dtype; P.res.o_sb = o_sb; P.res.o_sh = o_sh; P.res.Hq = Hq; P.res.mode = mode;
-        if (c->D == 128) decode8_row_kernel<128><<<dim3(Hq, B), 128, 0, ctx->stream>>>(P);
-        else decode8_row_kernel<64><<<dim3(Hq, B), 128, 0, ctx->stream>>>(P);
-        return launch_check(ctx, "decode8_row_kernel");
+        return decode8_launch(c, P, total, ex);
     }
     DecodeParams P{};
     P.q = q->data; P.q_dtype = q->dtype; P.q_sb = q->stride[0]; P.q_sh = q->stride[1];
@@ -1928,26 +1991,7 @@ static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fus
             decode_splitkv_kernel<64><<<grid, DEC_THREADS, smem, ctx->stream>>>(c->tmK, c->tmV, P);
         TRY(launch_check(ctx, "decode_splitkv_kernel"));
     }
-    // merge of the records of every (sequence, kv head) that was spread over several CTAs
-    CombineParams C{};
-    C.part_o = c->part_o; C.part_ml = c->part_ml; C.end = c->d_end;
-    C.B = B; C.Hkv = c->Hkv; C.g = g; C.D = c->D; C.grid = grid; C.res = P.res;
-    // record lanes per block: a kv head of a short sequence has one or two records, a 128 K-token sequence ~74
-    const long long per_head = longest * grid / std::max<long long>(1, total) + 2;
-    const int lanes = per_head <= 4 ? 2 : per_head <= 32 ? 8 : DEC_CL;
-    if (mode != 2) {
-        // (the kernel's blocks return at once for heads whose pages all went to one CTA)
-        decode_combine_kernel<<<dim3(Hq, B), (c->D / 4) * lanes, 0, ctx->stream>>>(C);
-        return launch_check(ctx, "decode_combine_kernel");
-    }
-    // KV-chunk decode over several GPUs: merge + exchange in one launch
-    CombineExchangeParams X{};
-    X.C = C;
-    exchange_targets(ex, &X.T);
-    exchange_merge_params(ex, &X.M, (int64_t)B * Hq, c->D, static_cast<float*>(out));
-    const unsigned blocks = (unsigned)std::min<long long>((long long)B * Hq, ctx->num_sms);
-    decode_combine_exchange_kernel<<<blocks, (c->D / 4) * lanes, 0, ctx->stream>>>(X);
-    return launch_check(ctx, "decode_combine_exchange_kernel");
+    return launch_combine(c, P.res, B, g, grid, total, longest, ex);
 }
 
 extern "C" int32_t fusor_cuda_flash_attention_decode(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* q,
