@@ -361,14 +361,10 @@ extern "C" int32_t fusor_cuda_ctx_create(int32_t device, void* stream, fusor_cud
         {(const void*)decode_splitkv_kernel<64>, 227 * 1024, "decode_splitkv_kernel<64>"},
         {(const void*)decode_cluster_kernel<128>, (int)DecodeClusterSmem<128>::bytes, "decode_cluster_kernel<128>"},
         {(const void*)decode_cluster_kernel<64>, (int)DecodeClusterSmem<64>::bytes, "decode_cluster_kernel<64>"},
-        {(const void*)decode8_splitkv_kernel<128, 1>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
-        {(const void*)decode8_splitkv_kernel<128, 2>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
-        {(const void*)decode8_splitkv_kernel<64, 1>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
-        {(const void*)decode8_splitkv_kernel<64, 2>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
-        {(const void*)decode8_cluster_kernel<128, 1>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
-        {(const void*)decode8_cluster_kernel<128, 2>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
-        {(const void*)decode8_cluster_kernel<64, 1>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
-        {(const void*)decode8_cluster_kernel<64, 2>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
+        {(const void*)decode8_splitkv_kernel<128>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
+        {(const void*)decode8_splitkv_kernel<64>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
+        {(const void*)decode8_cluster_kernel<128>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
+        {(const void*)decode8_cluster_kernel<64>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
         {(const void*)attn_mma16_kernel<96, false, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, false, true>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, true, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
@@ -1175,8 +1171,8 @@ extern "C" int32_t fusor_cuda_kvcache_create_dtype(fusor_cuda_ctx* ctx, int32_t 
     const bool i8 = dtype == FUSOR_CUDA_I8;
     const size_t rows = (size_t)num_pages * num_kv_heads * DEC_PT, pool_bytes = rows * head_dim * (i8 ? 1 : 2);
     void *k_pool = nullptr, *v_pool = nullptr;
-    c->max_grid = DEC_CTAS * ctx->num_sms;
-    c->max_slots = max_batch * num_kv_heads + c->max_grid;
+    c->max_grid = (i8 ? D8_CTAS : DEC_CTAS) * ctx->num_sms;
+    c->max_slots = max_batch * num_kv_heads + c->max_grid * (i8 ? D8_NW : 1);  // a record per (sequence, kv head) and CTA (8-bit: warp)
     auto alloc = [&](auto** p, size_t bytes) { return ctx->pool.plain(bytes, reinterpret_cast<void**>(p)); };
     bool ok = alloc(&k_pool, pool_bytes) == cudaSuccess && alloc(&v_pool, pool_bytes) == cudaSuccess &&
               (!i8 || alloc(&c->scales, rows * 2) == cudaSuccess) &&
@@ -1858,6 +1854,13 @@ static int32_t launch_combine(fusor_cuda_kvcache* c, const DecodeOutput& res, in
     // record lanes per block: a kv head of a short sequence has one or two records, a 128 K-token sequence ~74
     const long long per_head = longest * grid / std::max<long long>(1, total) + 2;
     const int lanes = per_head <= 4 ? 2 : per_head <= 32 ? 8 : DEC_CL;
+    if (res.mode != 2 && c->k_codes) {
+        const size_t smem = (size_t)(per_head + 3 + D8_MERGE / 32 * c->D) * 4;  // the weights of a head's records, and the warps' sums
+        const auto run = [&](auto kernel) { kernel<<<dim3(res.Hq, B), D8_MERGE, smem, ctx->stream>>>(C); };
+        if (c->D == 128) run(decode8_combine_kernel<128>);
+        else run(decode8_combine_kernel<64>);
+        return launch_check(ctx, "decode8_combine_kernel");
+    }
     if (res.mode != 2) {
         // (the kernel's blocks return at once for heads whose pages all went to one CTA)
         decode_combine_kernel<<<dim3(res.Hq, B), (c->D / 4) * lanes, 0, ctx->stream>>>(C);
@@ -1876,7 +1879,6 @@ static int32_t launch_combine(fusor_cuda_kvcache* c, const DecodeOutput& res, in
 // Decode over 8-bit pages, `total` (page, kv head) pairs in all: see decode8.cuh.
 static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, long long total, fusor_cuda_exchange* ex) {
     fusor_cuda_ctx* ctx = c->ctx;
-    const bool two = P.q_dtype == FUSOR_CUDA_F32;  // query terms
     long long longest = 0;
     for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
     const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;
@@ -1889,20 +1891,20 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
             cudaLaunchAttribute attr;
             const cudaLaunchConfig_t cfg = cluster_config(ctx, (unsigned)(heads * C), (unsigned)C, D8_THREADS,
                                                           c->D == 128 ? Decode8ClusterSmem<128>::bytes : Decode8ClusterSmem<64>::bytes, &attr);
-            CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, c->D == 128 ? (two ? decode8_cluster_kernel<128, 2> : decode8_cluster_kernel<128, 1>)
-                                                               : (two ? decode8_cluster_kernel<64, 2> : decode8_cluster_kernel<64, 1>), P, C));
+            CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, c->D == 128 ? decode8_cluster_kernel<128> : decode8_cluster_kernel<64>, P, C));
             return launch_check(ctx, "decode8_cluster_kernel");
         }
     }
-    const int per_sm = (int)std::max<long long>(1, std::min<long long>(D8_CTAS, total / (32 * ctx->num_sms)));
-    const int grid = (int)std::min<long long>(c->decode_ctas > 0 ? std::min(c->decode_ctas, c->max_grid) : per_sm * ctx->num_sms, total);
+    // every warp its share, at least a page of it
+    const int grid = c->decode_ctas > 0 ? c->decode_ctas : D8_CTAS * ctx->num_sms;
+    const int shares = (int)std::min<long long>((long long)grid * D8_NW, total);
     if (total > 0) {  // (every chunk empty: only the merge kernel runs and writes empty records)
-        const auto run = [&](auto kernel, size_t smem) { kernel<<<grid, D8_THREADS, smem, ctx->stream>>>(P); };
-        if (c->D == 128) run(two ? decode8_splitkv_kernel<128, 2> : decode8_splitkv_kernel<128, 1>, Decode8Smem<128>::bytes);
-        else run(two ? decode8_splitkv_kernel<64, 2> : decode8_splitkv_kernel<64, 1>, Decode8Smem<64>::bytes);
+        const auto run = [&](auto kernel, size_t smem) { kernel<<<(shares + D8_NW - 1) / D8_NW, D8_THREADS, smem, ctx->stream>>>(P, shares); };
+        if (c->D == 128) run(decode8_splitkv_kernel<128>, Decode8Smem<128>::bytes);
+        else run(decode8_splitkv_kernel<64>, Decode8Smem<64>::bytes);
         TRY(launch_check(ctx, "decode8_splitkv_kernel"));
     }
-    return launch_combine(c, P.res, P.B, P.g, grid, total, longest, ex);
+    return launch_combine(c, P.res, P.B, P.g, shares, total, longest, ex);
 }
 
 static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fusor_cuda_tensor4* q, float scale, void* out,
