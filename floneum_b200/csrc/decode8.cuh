@@ -21,9 +21,8 @@
 
 namespace fusor {
 
-constexpr int D8_NW = 8;      // warps of a CTA
+constexpr int D8_NW = 16;     // warps of a CTA
 constexpr int D8_SLOTS = 3;   // pages of a warp: one in use, two on their way
-constexpr int D8_CTAS = 2;    // CTAs per SM
 constexpr int D8_THREADS = D8_NW * 32;
 constexpr float D8_SHIFT = 6.0f;  // log2 of the factor the weights of value rows carry: with a page 2^8 above its reference 2^14
 
@@ -42,6 +41,7 @@ struct Decode8Params {
     float scale_log2;
     float* part_o;     // records as in DecodeParams
     float* part_ml;
+    int* done;         // [B * Hkv] pages whose records are written, zero between launches
     int* err;
     DecodeOutput res;
 };
@@ -49,11 +49,11 @@ struct Decode8Params {
 template <int D>
 struct Decode8Smem {
     static constexpr int TILE = DEC_PT * D;      // bytes of a page's K or V codes
-    static constexpr int SLOT = 2 * TILE;
+    static constexpr int SLOT = 2 * TILE + 128;  // K, V, 32 scales and padding: rows of K and V start on multiples of 64 or 128
     static constexpr int WARP = D8_SLOTS * SLOT;
-    static constexpr int SCALES = D8_NW * WARP;  // offset of [warp][slot][32]
-    static constexpr int META = SCALES + D8_NW * D8_SLOTS * 32;  // [warp][DEC_GP] float4, see Decode8State::store
-    static constexpr int bytes = META + D8_NW * DEC_GP * 16;
+    static constexpr int META = D8_NW * WARP;    // [warp][DEC_GP] float4, see Decode8State::store
+    static constexpr int WEIGHTS = META + D8_NW * DEC_GP * 16;  // the same: {of O, of the sum, largest score of the group, -}
+    static constexpr int bytes = WEIGHTS + D8_NW * DEC_GP * 16;
     static_assert(SLOT >= DEC_GP * D * 4, "a warp's output fits the slot it has just used");
 };
 
@@ -87,39 +87,43 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// Where a warp stands in a stream of pages: pages [0, n) of the stream are the pages of (b, hk) from 0 (the first: any) on, then
-// those of the next (b, hk) and so on.
+// A place in the pages of all (sequence, kv head) pairs, numbered in (b, hk, page) order and counted from where a warp's run begins.
 struct Decode8Walk {
     int b, hk;
     int np;   // pages of sequence b
-    int off;  // stream index of page 0 of (b, hk); negative in the first when the stream begins behind it
-    // to the (b, hk) that stream index i, inside the stream, belongs to
-    __device__ __forceinline__ void seek(const Decode8Params& P, int i) {
-        while (i >= off + np) {
-            off += np;
-            if (++hk < P.Hkv) continue;
-            hk = 0;
-            do {
-                ++b;
-                np = (__ldg(P.end + b) + DEC_PT - 1) / DEC_PT;
-            } while (np == 0);
-        }
+    int off;  // place of page 0 of (b, hk); negative when the run begins behind it
+    __device__ __forceinline__ void next(const Decode8Params& P) {  // the next pair that has pages (there is one)
+        off += np;
+        if (++hk < P.Hkv) return;
+        hk = 0;
+        do {
+            ++b;
+            np = (__ldg(P.end + b) + DEC_PT - 1) / DEC_PT;
+        } while (np == 0);
     }
 };
 
-// The pages of the stream a warp is about to copy, their table entries read two pages ahead of the copy.
+// The pages a warp is about to copy: every `step`-th of its run, their table entries read two pages ahead of the copy.
 struct Decode8Feed {
     Decode8Walk w;
-    int i, n, step;  // next stream index to look up, length of the stream, every which page of it
-    int page[2], hk[2];  // hk < 0: none
+    int i, n, step, seg_end;  // next page to look up, length of the run, where (b, hk) or the run ends
+    const int* entry;         // its place in the page table
+    int page[2], hk[2];       // hk < 0: none
+    __device__ __forceinline__ void seek(const Decode8Params& P) {
+        seg_end = min(n, w.off + w.np);
+        entry = P.page_table + (long long)w.b * P.max_pages + (i - w.off);
+    }
     __device__ __forceinline__ void look(const Decode8Params& P, int k) {
         hk[k] = -1;
-        if (i < n) {
-            w.seek(P, i);
-            hk[k] = w.hk;
-            page[k] = __ldg(P.page_table + (long long)w.b * P.max_pages + (i - w.off));  // first used by its copy
-            i += step;
+        if (i >= seg_end) {
+            if (i >= n) return;
+            w.next(P);
+            seek(P);
         }
+        hk[k] = w.hk;
+        page[k] = __ldg(entry);  // first used by its copy
+        entry += step;
+        i += step;
     }
     __device__ __forceinline__ void init(const Decode8Params& P, const Decode8Walk& start, int first, int length, int every) {
         w = start;
@@ -127,6 +131,7 @@ struct Decode8Feed {
         n = length;
         step = every;
         page[0] = page[1] = 0;
+        seek(P);
         look(P, 0);
         look(P, 1);
     }
@@ -136,32 +141,109 @@ struct Decode8Feed {
 template <int D>
 __device__ __forceinline__ int d8_swizzle(int row) { return D == 128 ? row & 7 : (row >> 1) & 3; }
 
-// The next page of the feed into a slot, as a group of its own (an empty one when there is none).
+// Where a lane reads fragments of a tile (of chunks 0 and 1; chunk pair c is the place ^ 16 c) and writes its chunks (the first; the next
+// is 512 bytes on, its chunk the first's ^ 4 for rows of 128 bytes, the same for rows of 64).
 template <int D>
-__device__ __forceinline__ void d8_copy(const Decode8Params& P, Decode8Feed& F, uint32_t slot, uint32_t scale_slot, int lane) {
+__device__ __forceinline__ uint32_t d8_frag(int lane) { return (lane & 15) * D + (((lane >> 4) ^ d8_swizzle<D>(lane & 15)) << 4); }
+template <int D>
+__device__ __forceinline__ uint32_t d8_place(int lane) {
     constexpr int CH = D / 16;  // 16-byte chunks of a row
+    return lane / CH * D + (((lane % CH) ^ d8_swizzle<D>(lane / CH)) << 4);
+}
+
+// The next page of the feed into a slot, as a group of its own (an empty one when there is none).  place: slot + d8_place.
+template <int D>
+__device__ __forceinline__ void d8_copy(const Decode8Params& P, Decode8Feed& F, uint32_t place, uint32_t scale_slot, int lane) {
+    constexpr int TILE = DEC_PT * D;
     if (F.hk[0] >= 0) {
         int page = F.page[0];
         if ((unsigned)page >= (unsigned)P.num_pages) {  // record and read page 0 instead
             if (lane == 0) atomicExch(P.err, kErrBadPage);
             page = 0;
         }
-        const long long tile = (long long)page * P.Hkv + F.hk[0];
-        const int8_t* k = P.k_codes + tile * (DEC_PT * D) + lane * 16;
-        const int8_t* v = P.v_codes + tile * (DEC_PT * D) + lane * 16;
+        const uint32_t tile = (uint32_t)page * (uint32_t)P.Hkv + (uint32_t)F.hk[0];  // (the pool has fewer than 2^31 rows of 16)
+        const unsigned long long at = (unsigned long long)tile * TILE + lane * 16;
+        const int8_t *k = P.k_codes + at, *v = P.v_codes + at;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-            const int row = lane / CH + j * (32 / CH);
-            const uint32_t dst = slot + row * D + ((lane % CH) ^ d8_swizzle<D>(row)) * 16;
+            const uint32_t dst = (D == 128 && (j & 1) ? place ^ 64 : place) + j * 512;
             cp_async16(dst, k + j * 512);
-            cp_async16(dst + DEC_PT * D, v + j * 512);
+            cp_async16(dst + TILE, v + j * 512);
         }
-        if (lane < 2) cp_async16(scale_slot + lane * 16, P.scales + tile * 32 + lane * 16);
+        if (lane < 2) cp_async16(scale_slot + lane * 16, P.scales + (unsigned long long)tile * 32 + lane * 16);
     }
     cp_async_commit();
     F.page[0] = F.page[1];
     F.hk[0] = F.hk[1];
     F.look(P, 1);
+}
+
+// The query heads of a (sequence, kv head) as digits, [digit][head][ROW] words of four dims, then what turns a sum of digits times codes
+// into a score in log2 units, but for the row's step, per head.  (Padded rows: the fragments' reads meet no bank conflict.)
+template <int D>
+struct Decode8Digits {
+    static constexpr int ROW = D / 4 + 4, WORDS = 3 * DEC_GP * ROW + DEC_GP;
+    static_assert(WORDS * 4 <= Decode8Smem<D>::SLOT, "they fit a slot");
+};
+
+// Query heads first, first + step, .. of the group into `digits`, a warp; D = 64: two at a time.  Heads past the last: factor 0, and
+// whatever lies there as digits (whole numbers, so their scores are zeros).
+template <int D>
+__device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk, int first, int step, uint32_t* digits, int lane) {
+    constexpr int PER = 128 / D, ROW = Decode8Digits<D>::ROW;  // heads at a time
+    const int word = lane % (D / 4), sub = lane / (D / 4);
+    const unsigned mates = D == 128 ? 0xffffffffu : 0xffffu << (16 * sub);
+    if (first == 0 && lane >= P.g && lane < DEC_GP) digits[3 * DEC_GP * ROW + lane] = 0u;
+    for (int h0 = first * PER; h0 < P.g; h0 += 2 * step * PER) {
+        uint32_t raw[2][4] = {};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int h = h0 + u * step * PER + sub;
+            if (h >= P.g) continue;
+            const long long at = b * P.q_sb + (long long)(hk * P.g + h) * P.q_sh + 4 * word;
+            if (P.q_dtype == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raw[u][e] = __ldg(static_cast<const uint32_t*>(P.q) + at + e);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) raw[u][e] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(P.q) + at) + e);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int h = h0 + u * step * PER + sub;
+            if (h0 + u * step * PER >= P.g) break;
+            float x[4];
+            if (P.q_dtype == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[u][e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 f = P.q_dtype == 1 ? make_float2(__uint_as_float(raw[u][e] << 16), __uint_as_float(raw[u][e] & 0xffff0000u))
+                                                    : __half22float2(*reinterpret_cast<const __half2*>(&raw[u][e]));
+                    x[2 * e] = f.x;
+                    x[2 * e + 1] = f.y;
+                }
+            }
+            const uint32_t big = __reduce_max_sync(mates, max(max(abs_bits(x[0]), abs_bits(x[1])), max(abs_bits(x[2]), abs_bits(x[3]))));
+            // 2^up q is at most 126 * 2^16 (up at most 100: the factor back stays a normal number)
+            const int up = min(16 + 133 - (int)((big + 0x20000u) >> 23), 100);
+            const float factor = __uint_as_float((uint32_t)(127 + up) << 23);
+            uint32_t n[4];  // with 128 added to each digit they are the bytes; flipping the top bit takes it off again
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n[e] = (uint32_t)(__float2int_rn(x[e] * factor) + 0x808080);
+            const uint32_t lo01 = __byte_perm(n[0], n[1], 0x5140), lo23 = __byte_perm(n[2], n[3], 0x5140);
+            const uint32_t hi = __byte_perm(__byte_perm(n[0], n[1], 0x0062), __byte_perm(n[2], n[3], 0x0062), 0x5410);
+            uint32_t* out = digits + h * ROW + word;
+            out[0] = hi ^ 0x80808080u;
+            out[DEC_GP * ROW] = __byte_perm(lo01, lo23, 0x7632) ^ 0x80808080u;
+            out[2 * DEC_GP * ROW] = __byte_perm(lo01, lo23, 0x5410) ^ 0x80808080u;
+            // a query that is not finite: NaN in every place of its head's result
+            const float back = big >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : P.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+            if (word == 0 && h < P.g) digits[3 * DEC_GP * ROW + h] = __float_as_uint(back);
+        }
+    }
 }
 
 // A warp's state over one (sequence, kv head).  A lane holds columns (query heads) 2 (lane % 4) and the next.
@@ -174,50 +256,17 @@ struct Decode8State {
     float l[2];
     float o[D / 16][4];        // [dims 16 c + 2 (lane / 4), next][columns]: (d, col), (d, col + 1), (d + 1, col), (d + 1, col + 1)
 
-    __device__ __forceinline__ void load_q(const Decode8Params& P, int b, int hk, int lane) {
-        const int h = lane >> 2, t = lane & 3;
-        float x[D / 16][4];
-        uint32_t big = 0;
-        const long long at = b * P.q_sb + (long long)(hk * P.g + h) * P.q_sh + 4 * t;
+    // The query from what d8_digits has left in shared memory, and the state before the first page.
+    __device__ __forceinline__ void start(const uint32_t* digits, int lane) {
+        constexpr int ROW = Decode8Digits<D>::ROW;
+        const int t = lane & 3;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-            if (P.q_dtype == 0) {
+        for (int k = 0; k < 3; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[c][e] = h < P.g ? __ldg(static_cast<const float*>(P.q) + at + 16 * c + e) : 0.0f;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const uint32_t u = h < P.g ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(P.q) + at + 16 * c + e)) : 0;
-                    const float2 f = P.q_dtype == 1 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u))
-                                                    : __half22float2(*reinterpret_cast<const __half2*>(&u));
-                    x[c][e] = f.x;
-                    x[c][e + 1] = f.y;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) big = max(big, abs_bits(x[c][e]));
-        }
-        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        // 2^up q is at most 126 * 2^16 (up at most 100: the factor back stays a normal number)
-        const int up = min(16 + 133 - (int)((big + 0x20000u) >> 23), 100);
-        const float factor = __uint_as_float((uint32_t)(127 + up) << 23);
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-            uint32_t u[4];  // with 128 added to each digit they are the bytes; flipping the top bit takes it off again
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] = (uint32_t)(__float2int_rn(x[c][e] * factor) + 0x808080);
-            const uint32_t lo01 = __byte_perm(u[0], u[1], 0x5140), lo23 = __byte_perm(u[2], u[3], 0x5140);
-            q[2][c >> 1][c & 1] = __byte_perm(lo01, lo23, 0x5410) ^ 0x80808080u;
-            q[1][c >> 1][c & 1] = __byte_perm(lo01, lo23, 0x7632) ^ 0x80808080u;
-            q[0][c >> 1][c & 1] = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410) ^ 0x80808080u;
-        }
-        // a query that is not finite: NaN in every place of its head's result
-        const float back = h >= P.g ? 0.0f : big >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : P.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-        qs[0] = __shfl_sync(0xffffffffu, back, 8 * t);
-        qs[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+            for (int c = 0; c < D / 16; ++c) q[k][c >> 1][c & 1] = digits[(k * DEC_GP + (lane >> 2)) * ROW + 4 * c + t];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            qs[j] = __uint_as_float(digits[3 * DEC_GP * ROW + 2 * t + j]);
             top[j] = -INFINITY;
             m[j] = mv[j] = -FLT_MAX;  // (finite: -inf - m is -inf)
             l[j] = 0.0f;
@@ -227,10 +276,10 @@ struct Decode8State {
     }
 
     // One page in shared memory, tokens tok0 .. tok0 + 15 of which 0 .. len - 1 exist.  Whole warp.
-    __device__ __forceinline__ void page(uint32_t slot, uint32_t scale_slot, int tok0, int len, int lane) {
+    // frag: slot + d8_frag.
+    __device__ __forceinline__ void page(uint32_t frag, uint32_t scale_slot, int tok0, int len, int lane) {
         constexpr int TILE = DEC_PT * D;
-        const int row = lane & 15, gl = lane >> 2;
-        const uint32_t kb = slot + row * D, sw = d8_swizzle<D>(row), half = lane >> 4;
+        const int gl = lane >> 2;
         // ---- the page's scales, one per lane: steps of K, exponents of V
         uint32_t byte;
         asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_slot + lane) : "memory");
@@ -239,7 +288,7 @@ struct Decode8State {
 #pragma unroll
         for (int c = 0; c < D / 16; c += 2) {
             uint32_t a[4];
-            ldmatrix_x4(a, kb + (((c + half) ^ sw) << 4));
+            ldmatrix_x4(a, frag ^ (c << 4));
 #pragma unroll
             for (int k = 0; k < 3; ++k) mma_s8_16832(acc[k], a, q[k][c >> 1][0], q[k][c >> 1][1]);
         }
@@ -310,7 +359,7 @@ struct Decode8State {
 #pragma unroll
         for (int c = 0; c < D / 16; c += 2) {
             uint32_t v[4];
-            ldmatrix_x4_trans(v, kb + TILE + (((c + half) ^ sw) << 4));
+            ldmatrix_x4_trans(v, (frag ^ (c << 4)) + TILE);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint32_t a[4] = {codes_f16(v[2 * u]), codes_f16(v[2 * u] >> 8), codes_f16(v[2 * u + 1]), codes_f16(v[2 * u + 1] >> 8)};
@@ -342,9 +391,11 @@ struct Decode8State {
         }
     }
 
-    // The reduced state to shared memory: O [DEC_GP][D] and per column {largest score, sum, reference of the output, -}.
-    __device__ __forceinline__ void store(float* out, float4* meta, int lane) const {
+    // The reduced state to shared memory, over the warp's slots: O [DEC_GP][D] and per column {largest score, sum, reference of the output, -}.
+    __device__ __forceinline__ void store(uint8_t* smem, int warp, int lane) const {
         const int gl = lane >> 2, t = lane & 3;
+        float* out = reinterpret_cast<float*>(smem + warp * Decode8Smem<D>::WARP);
+        float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D>::META) + warp * DEC_GP;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (gl == 0) meta[2 * t + j] = make_float4(m[j], l[j], mv[j] - D8_SHIFT, 0.0f);
@@ -393,46 +444,191 @@ struct Decode8State {
     }
 };
 
-// The warps' states merged, for query head rr of the group and dims 4 dg .. 4 dg + 3.  out(w): a warp's O.
-template <int D, class Out>
-__device__ __forceinline__ void d8_merge(const float4* meta, Out out, int rr, int dg, float& M, float& L, float4& acc) {
-    M = -INFINITY;
-    L = 0.0f;
-    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+// T pages dealt to `shares` as [c T / shares, (c + 1) T / shares): decode_walk_init's and decode_page_owner's numbers without 64-bit
+// divisions (a few hundred cycles each, at both ends of a kernel of some microseconds).
+struct Decode8Deal {
+    int T, shares, each, rest;
+    __device__ __forceinline__ Decode8Deal(int pages, int n) : T(pages), shares(n), each(pages / n), rest(pages % n) {}
+    __device__ __forceinline__ int bound(int c) const {  // first page of share c; rest < shares < 2^12
+        c = min(c, shares);
+        return c * each + (int)((unsigned)(c * rest) / (unsigned)shares);
+    }
+    __device__ __forceinline__ int owner(int page) const {  // floor(((page + 1) shares - 1) / T): an estimate, off by one at most
+        const long long x = (long long)(page + 1) * shares - 1;
+        int q = (int)((float)(page + 1) * (float)shares / (float)T);
+        long long r = x - (long long)q * T;
+        while (r < 0) { --q; r += T; }
+        while (r >= T) { ++q; r -= T; }
+        return q;
+    }
+};
+
+// A warp's slots: pages come in turn, two ahead of the one in use.
+template <int D>
+struct Decode8Ring {
+    static constexpr uint32_t SLOT = Decode8Smem<D>::SLOT, LAST = (D8_SLOTS - 1) * SLOT;
+    uint32_t base, frag, place;  // of slot 0
+    uint32_t now, spare;         // offsets of the slot of the next page, and of the one that holds nothing that is still needed
+    __device__ __forceinline__ Decode8Ring(const void* smem, int warp, int lane)
+        : base(smem_u32(smem) + warp * Decode8Smem<D>::WARP), frag(base + d8_frag<D>(lane)), place(base + d8_place<D>(lane)), now(0), spare(LAST) {}
+    __device__ __forceinline__ void fill(const Decode8Params& P, Decode8Feed& feed, int lane) {
 #pragma unroll
-    for (int w = 0; w < D8_NW; ++w) M = fmaxf(M, meta[w * DEC_GP + rr].x);
+        for (uint32_t at = 0; at < LAST; at += SLOT) d8_copy<D>(P, feed, place + at, base + at + 2 * DEC_PT * D, lane);
+    }
+    __device__ __forceinline__ void page(const Decode8Params& P, Decode8Feed& feed, Decode8State<D>& st, int tok0, int len, int lane) {
+        cp_async_wait<D8_SLOTS - 2>();
+        __syncwarp();  // the page is there, and every lane is done with the slot before it
+        d8_copy<D>(P, feed, place + spare, base + spare + 2 * DEC_PT * D, lane);
+        st.page(frag + now, base + now + 2 * DEC_PT * D, tok0, len, lane);
+        spare = now;
+        now = now == LAST ? 0 : now + SLOT;
+    }
+};
+
+// The CTA's merge of its warps' states (Decode8State::store has put them at smem + w * WARP and to meta).  ends_with[w]: which warps belong
+// together, neighbours; < 0: none.  First every (warp, head) its weight next to its group's largest score, then the sums, where nothing
+// waits for anything.  done(w0, group size, rr, dg, M, L, acc) gets the group's first warp and the sums of dims 4 dg .. 4 dg + 3.
+template <int D, class Done>
+__device__ __forceinline__ void d8_merge_warps(uint8_t* smem, const int* ends_with, int g, Done done) {
+    float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D>::META);
+    float4* weights = reinterpret_cast<float4*>(smem + Decode8Smem<D>::WEIGHTS);
+    const int tid = threadIdx.x, lane = tid & 31;
+    __syncthreads();
+    const int pair = lane < D8_NW ? ends_with[lane] : -1, before = __shfl_up_sync(0xffffffffu, pair, 1);
+    const unsigned joins = __ballot_sync(0xffffffffu, lane > 0 && pair >= 0 && pair == before);  // warps that go with the one before
+    const unsigned leads = __ballot_sync(0xffffffffu, pair >= 0) & ~joins;
+    const auto size_of = [&](int w0) { return __ffs(~(joins >> (w0 + 1))); };
+    if (tid < D8_NW * DEC_GP) {
+        const int w = tid / DEC_GP, rr = tid % DEC_GP;
+        const unsigned upto = leads & ((2u << w) - 1);  // the last of them is this warp's group's, if it has one
+        const int w0 = 31 - __clz(upto | 1);
+        if (rr < g && upto && w < w0 + size_of(w0)) {
+            const float4 mine = meta[w * DEC_GP + rr];
+            float M = -INFINITY;
+            for (int k = w0; k < w0 + size_of(w0); ++k) M = fmaxf(M, meta[k * DEC_GP + rr].x);
+            const bool none = mine.y == 0.0f;  // no page
+            weights[w * DEC_GP + rr] = make_float4(none ? 0.0f : fast_exp2(mine.z - M), none ? 0.0f : mine.y * fast_exp2(mine.x - M), M, 0.0f);
+        }
+    }
+    __syncthreads();
+    const int items = __popc(leads) * g * (D / 4);
+    for (int item = tid; item < items; item += D8_THREADS) {
+        const int dg = item % (D / 4), row = item / (D / 4), rr = row % g;
+        unsigned from = leads;
+        for (int k = row / g; k > 0; --k) from &= from - 1;
+        const int w0 = __ffs(from) - 1, size = size_of(w0);
+        const uint8_t* state = smem + w0 * Decode8Smem<D>::WARP + (rr * D + dg * 4) * 4;
+        const float4* weight = weights + w0 * DEC_GP + rr;
+        const float M = weight->z;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float L = 0.0f;
+        for (int k = 0; k < size; k += 4) {
 #pragma unroll
-    for (int w = 0; w < D8_NW; ++w) {
-        const float4 x = meta[w * DEC_GP + rr];
-        if (x.y == 0.0f) continue;  // no page
-        const float a = fast_exp2(x.z - M);
-        const float4 o = *reinterpret_cast<const float4*>(out(w) + rr * D + dg * 4);
-        acc.x += a * o.x; acc.y += a * o.y; acc.z += a * o.z; acc.w += a * o.w;
-        L += x.y * fast_exp2(x.x - M);
+            for (int u = 0; u < 4; ++u) {
+                const int at = min(k + u, size - 1);
+                const float2 x = k + u < size ? *reinterpret_cast<const float2*>(weight + at * DEC_GP) : make_float2(0.0f, 0.0f);
+                const float4 o = *reinterpret_cast<const float4*>(state + at * Decode8Smem<D>::WARP);
+                L += x.y;
+                acc.x += x.x * o.x; acc.y += x.x * o.y; acc.z += x.x * o.z; acc.w += x.x * o.w;
+            }
+        }
+        done(w0, size, rr, dg, M, L, acc);
+    }
+}
+
+// The records of a (sequence, kv head) whose pages are [page0, page0 + np) of T, when more than one share has pages of it: one for each
+// CTA in which it is what shares end with, in the slot of the first of them, and one of the share that it ends inside of, if any.
+struct Decode8Records {
+    int c_first, c_last;  // its shares
+    int cta, groups, n;   // CTA of the first share; CTAs with a record of their shares; records
+    Decode8Records() = default;
+    __device__ __forceinline__ Decode8Records(const Decode8Deal& deal, int page0, int np) {
+        c_first = deal.owner(page0);
+        c_last = deal.owner(page0 + np - 1);
+        const int inside = deal.bound(c_last + 1) > page0 + np;
+        cta = c_first / D8_NW;
+        groups = (c_last - inside) / D8_NW - cta + 1;
+        n = groups + inside;
+    }
+    __device__ __forceinline__ int share(int i) const { return i == 0 ? c_first : i < groups ? (cta + i) * D8_NW : c_last; }
+};
+
+// One query head's records merged to its result, by a warp; other CTAs have written them, so nothing of them is read from L1.  The loads
+// of eight records do not wait for their weights.
+template <int D>
+__device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const Decode8Records& R, int pair, int rr, int lane) {
+    constexpr int E = D / 32, BATCH = 8;
+    const int b = pair / P.Hkv, hk = pair % P.Hkv;
+    float M = -INFINITY, L = 0.0f, acc[E] = {};
+    for (int i0 = 0; i0 < R.n; i0 += BATCH) {
+        const int here = min(BATCH, R.n - i0);
+        const long long row = (long long)(pair + R.share(i0 + min(lane, here - 1))) * DEC_GP + rr;
+        const float2 x = lane < here ? __ldcg(reinterpret_cast<const float2*>(P.part_ml) + row) : make_float2(-INFINITY, 0.0f);
+        float o[BATCH][E];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const float* from = P.part_o + __shfl_sync(0xffffffffu, row, k) * D + lane * E;  // (past the last record: the last one's)
+            if (k < here) {
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(from + e));
+                    o[k][e] = y.x;
+                    o[k][e + 1] = y.y;
+                }
+            }
+        }
+        float top = x.x;
+#pragma unroll
+        for (int z = 16; z > 0; z >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+        top = fmaxf(M, top);
+        const float weight = x.y == 0.0f ? 0.0f : fast_exp2(x.x - top), before = M == -INFINITY ? 0.0f : fast_exp2(M - top);
+        M = top;
+        L = L * before + (x.y == 0.0f ? 0.0f : weight * x.y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= before;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const float a = __shfl_sync(0xffffffffu, weight, k);
+            if (k < here && a != 0.0f) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += a * o[k][e];
+            }
+        }
+    }
+#pragma unroll
+    for (int z = 16; z > 0; z >>= 1) L += __shfl_xor_sync(0xffffffffu, L, z);
+    if (E == 4) {
+        decode_emit(P.res, D, P.g, b, hk, rr, lane, M, L, make_float4(acc[0], acc[1], acc[E - 2], acc[E - 1]));
+    } else {
+        const float z = __shfl_down_sync(0xffffffffu, acc[0], 1), w = __shfl_down_sync(0xffffffffu, acc[1], 1);
+        if (!(lane & 1)) decode_emit(P.res, D, P.g, b, hk, rr, lane >> 1, M, L, make_float4(acc[0], acc[1], z, w));
     }
 }
 
 // The pages of all (sequence, kv head) pairs, numbered as in decode_splitkv_kernel, are dealt evenly to `shares` warps, each a run of
-// its own: warps meet nobody on the way, copies run on over the ends of sequences, and what a warp has of a (sequence, kv head) goes
-// from its registers to the result, when it is all of it, or to a record for decode_combine_kernel (to which a share is what
-// a CTA is there).  Only the warps of a CTA that lies inside one (sequence, kv head) merge their states first and write one record, the
-// first warp's, so that a long sequence has a record per CTA.
+// its own: warps meet nobody on the way, copies run on over the ends of sequences, and a pair that a warp has all pages of goes from
+// its registers to the result.  What a warp ends with is merged with the warps of the CTA that end with the same pair, to one
+// record.  Then the CTA adds the pages it had of each pair to a counter, and merges the records of those that are complete with
+// it: no second launch, and no order of arrival in a result.
 template <int D>
-__global__ void __launch_bounds__(D8_THREADS, D8_CTAS) decode8_splitkv_kernel(const __grid_constant__ Decode8Params P, const int shares) {
+__global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __grid_constant__ Decode8Params P, const int shares) {
     using Smem = Decode8Smem<D>;
     extern __shared__ __align__(128) uint8_t d8_smem[];
+    __shared__ int ends_with[D8_NW];  // the pair that a warp's last pages belong to, -1 when there is nothing to merge
+    __shared__ int4 parts[2 * D8_NW]; // what a warp begins and ends with, when it has not all of it: {pair, first page of it, pages here, pages}
+    __shared__ struct { int pair; Decode8Records records; } complete[2 * D8_NW];
+    __shared__ int n_complete;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cta0 = (int)blockIdx.x * D8_NW, share = cta0 + warp;
     // T pages in all
     int sum = 0;
     for (int b0 = 0; b0 < P.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < P.B ? (P.end[b0 + lane] + DEC_PT - 1) / DEC_PT : 0);
     const int T = sum * P.Hkv;
-    const auto bound = [&](int c) { return (int)((long long)min(c, shares) * T / shares); };
-    const int cta_first = bound(cta0), cta_end = bound(cta0 + D8_NW);
-    const int first = min(bound(share), cta_end - 1), n = bound(share + 1) - bound(share);  // (a share has a page at least; warps past the last: n = 0)
+    const Decode8Deal deal(T, shares);
+    const int first = deal.bound(share), n = deal.bound(share + 1) - first;  // (a share has a page at least; warps past the last: none)
     // the sequence that holds the warp's first page, and the pages (per kv head) before it
-    Decode8Walk w;
-    for (int b0 = 0, cum = 0;; b0 += 32) {
+    Decode8Walk w{};
+    for (int b0 = 0, cum = 0; n > 0; b0 += 32) {
         const int pages = b0 + lane < P.B ? (P.end[b0 + lane] + DEC_PT - 1) / DEC_PT : 0;
         int upto = pages;
 #pragma unroll
@@ -452,135 +648,73 @@ __global__ void __launch_bounds__(D8_THREADS, D8_CTAS) decode8_splitkv_kernel(co
         }
         cum += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const bool together = cta_first >= first + w.off && cta_end <= first + w.off + w.np && shares - cta0 > 1;
-    if (n == 0 && !together) return;
-    const uint32_t ring = smem_u32(d8_smem) + warp * Smem::WARP, scales = smem_u32(d8_smem) + Smem::SCALES + warp * D8_SLOTS * 32;
+    Decode8Ring<D> ring(d8_smem, warp, lane);
     Decode8Feed feed;
     feed.init(P, w, 0, n, 1);
-    d8_copy<D>(P, feed, ring, scales, lane);
-    d8_copy<D>(P, feed, ring + Smem::SLOT, scales + 32, lane);
+    ring.fill(P, feed, lane);
 
+    if (P.res.mode == 1)  // sequences without pages: empty records
+        for (int row = (int)blockIdx.x * D8_THREADS + tid; row < P.B * P.res.Hq; row += gridDim.x * D8_THREADS)
+            if (P.end[row / P.res.Hq] == 0) {
+                float* r = static_cast<float*>(P.res.out) + (long long)row * (D + 2);
+                r[0] = -INFINITY;
+                for (int d = 1; d < D + 2; ++d) r[d] = 0.0f;
+            }
+    if (tid == 0) n_complete = 0;
+    if (lane < 2) parts[2 * warp + lane] = make_int4(0, 0, 0, 0);
     Decode8State<D> st;
-    int i = 0, slot = 0, free_slot = 2;  // the next page, its slot, and the one that holds nothing that is still needed
-    do {
-        if (n > 0) w.seek(P, i);
+    int open = -1;
+    for (int i = 0; i < n; w.next(P)) {
         const int seg_end = min(n, w.off + w.np);
         const int front = __ldg(P.front + w.b), len = __ldg(P.end + w.b) - front;
-        st.load_q(P, w.b, w.hk, lane);
-        for (; i < seg_end; ++i) {
-            cp_async_wait<1>();
-            __syncwarp();  // the page is there, and every lane is done with the slot before it
-            d8_copy<D>(P, feed, ring + free_slot * Smem::SLOT, scales + free_slot * 32, lane);
-            st.page(ring + slot * Smem::SLOT, scales + slot * 32, (i - w.off) * DEC_PT - front, len, lane);
-            free_slot = slot;
-            slot = slot == D8_SLOTS - 1 ? 0 : slot + 1;
-        }
+        uint32_t* digits = reinterpret_cast<uint32_t*>(d8_smem + warp * Smem::WARP + ring.spare);
+        __syncwarp();  // every lane is done with the slot
+        d8_digits<D>(P, w.b, w.hk, 0, 1, digits, lane);
+        __syncwarp();
+        st.start(digits, lane);
+        for (int tok0 = (i - w.off) * DEC_PT - front; i < seg_end; ++i, tok0 += DEC_PT) ring.page(P, feed, st, tok0, len, lane);
         st.reduce();
-        if (!together)
-            st.emit(P, w.b, w.hk, w.off >= 0 && w.off + w.np <= n && P.res.mode != 2, (long long)w.b * P.Hkv + w.hk + share, lane);
-    } while (i < n);
-    if (!together) return;
-
-    cp_async_wait<0>();
-    __syncwarp();
-    float4* meta = reinterpret_cast<float4*>(d8_smem + Smem::META);
-    const auto out = [&](int k) { return reinterpret_cast<float*>(d8_smem + k * Smem::WARP); };  // nothing is on its way any more
-    st.store(out(warp), meta + warp * DEC_GP, lane);
-    __syncthreads();
-    const long long rec = (long long)w.b * P.Hkv + w.hk + cta0;
-    for (int item = tid; item < P.g * (D / 4); item += D8_THREADS) {
-        const int rr = item / (D / 4), dg = item % (D / 4);
-        float M, L;
-        float4 acc;
-        d8_merge<D>(meta, out, rr, dg, M, L, acc);
-        *reinterpret_cast<float4*>(P.part_o + (rec * DEC_GP + rr) * D + dg * 4) = acc;
+        const int pair = w.b * P.Hkv + w.hk;
+        const bool whole = w.off >= 0 && w.off + w.np <= n && P.res.mode != 2;
+        if (!whole && lane == 0) parts[2 * warp + (i >= n)] = make_int4(pair, first + w.off, seg_end - max(0, w.off), w.np);
+        if (whole || i < n) {
+            st.emit(P, w.b, w.hk, whole, (long long)pair + share, lane);
+        } else {
+            cp_async_wait<0>();
+            __syncwarp();  // nothing is on its way to the slots any more
+            st.store(d8_smem, warp, lane);
+            open = pair;
+        }
+        if (i >= n) break;
+    }
+    if (lane == 0) ends_with[warp] = open;
+    d8_merge_warps<D>(d8_smem, ends_with, P.g, [&](int w0, int size, int rr, int dg, float M, float L, float4 acc) {
+        const long long rec = ((long long)ends_with[w0] + cta0 + w0) * DEC_GP + rr;
+        *reinterpret_cast<float4*>(P.part_o + rec * D + dg * 4) = acc;
         if (dg == 0) {
-            *reinterpret_cast<float2*>(P.part_ml + (rec * DEC_GP + rr) * 2) = make_float2(M, L);
-            for (int k = 1; k < D8_NW && cta0 + k < shares; ++k)  // the other warps' records: empty
-                *reinterpret_cast<float2*>(P.part_ml + ((rec + k) * DEC_GP + rr) * 2) = make_float2(-INFINITY, 0.0f);
+            *reinterpret_cast<float2*>(P.part_ml + rec * 2) = make_float2(M, L);
+            if (P.res.mode == 2)  // its merge looks at a record of every share
+                for (int k = 1; k < size; ++k) *reinterpret_cast<float2*>(P.part_ml + (rec + k * DEC_GP) * 2) = make_float2(-INFINITY, 0.0f);
         }
-    }
-}
+    });
+    if (P.res.mode == 2) return;
 
-// One block per (query head, sequence), whose records may be hundreds, most of them empty: the weights of all records first, in two
-// rounds of loads whatever their number, then the sums, a run of records per warp and no load of an empty one.  A head whose pages all went to one warp has been written by that warp.
-constexpr int D8_MERGE = 256;  // threads
-template <int D>
-__global__ void __launch_bounds__(D8_MERGE) decode8_combine_kernel(const __grid_constant__ CombineParams P) {
-    extern __shared__ __align__(16) float d8_weight[];  // [records], then [warps][D]
-    __shared__ int red[66];
-    __shared__ float part[2][D8_MERGE / 32];
-    const int h = blockIdx.x, b = blockIdx.y, hk = h / P.g, rr = h % P.g, tid = threadIdx.x, warp = tid >> 5;
-    int first, n;
-    decode_head_records(P.end, P.B, P.Hkv, P.grid, b, hk, red, first, n);
-    if (n == 1) return;
-    float2 ml[4];  // this thread's records, where four a thread are enough; else they are read again
-    float M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int s = tid + k * D8_MERGE;
-        ml[k] = s < n ? *reinterpret_cast<const float2*>(P.part_ml + ((long long)(first + s) * DEC_GP + rr) * 2) : make_float2(-INFINITY, 0.0f);
-        M = fmaxf(M, ml[k].x);
-    }
-    for (int s = tid + 4 * D8_MERGE; s < n; s += D8_MERGE) M = fmaxf(M, P.part_ml[((long long)(first + s) * DEC_GP + rr) * 2]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    if ((tid & 31) == 0) part[0][warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < D8_MERGE / 32; ++w) M = fmaxf(M, part[0][w]);
-    float L = 0.0f;
-    const auto weigh = [&](int s, float2 x) {
-        const float a = x.y == 0.0f ? 0.0f : fast_exp2(x.x - M);
-        d8_weight[s] = a;
-        if (x.y != 0.0f) L += a * x.y;
-    };
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (tid + k * D8_MERGE < n) weigh(tid + k * D8_MERGE, ml[k]);
-    for (int s = tid + 4 * D8_MERGE; s < n; s += D8_MERGE) weigh(s, *reinterpret_cast<const float2*>(P.part_ml + ((long long)(first + s) * DEC_GP + rr) * 2));
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-    if ((tid & 31) == 0) part[1][warp] = L;
-    __syncthreads();
-    L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < D8_MERGE / 32; ++w) L += part[1][w];
-    // a run of records per warp, the loads of four that are not empty at a time
-    constexpr int NW = D8_MERGE / 32, E = D / 32;
-    const int lane = tid & 31, end = (int)((long long)n * (warp + 1) / NW);
-    float acc[E] = {};
-    const float* po = P.part_o + ((long long)first * DEC_GP + rr) * D + lane * E;
-    for (int s0 = (int)((long long)n * warp / NW); s0 < end; s0 += 32) {
-        unsigned some = __ballot_sync(0xffffffffu, s0 + lane < end && d8_weight[s0 + lane] != 0.0f);
-        while (some) {
-            float a[4], o[4][E];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int s = s0 + __ffs(some) - 1;
-                a[k] = some ? d8_weight[s] : 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[k][e] = some ? po[(long long)s * (DEC_GP * D) + e] : 0.0f;
-                some &= some - 1;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += a[k] * o[k][e];
+    // ---- the pairs that are complete with this CTA's pages
+    __threadfence();
+    __syncthreads();  // this CTA's records can be seen everywhere
+    if (tid < 2 * D8_NW && parts[tid].z > 0) {
+        const int4 part = parts[tid];
+        const int pair = part.x, before = atomicAdd(P.done + pair, part.z);
+        const Decode8Records R(deal, part.y, part.w);
+        if (before + part.z == part.w) {
+            P.done[pair] = 0;
+            complete[atomicAdd(&n_complete, 1)] = {pair, R};
         }
     }
-    float* sum = d8_weight + (n + 3) / 4 * 4;  // [warp][D]
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[warp * D + lane * E + e] = acc[e];
+    __threadfence();
     __syncthreads();
-    if (tid >= D / 4) return;
-    float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float4 o = *reinterpret_cast<const float4*>(sum + w * D + tid * 4);
-        all.x += o.x; all.y += o.y; all.z += o.z; all.w += o.w;
-    }
-    decode_emit(P.res, D, P.g, b, hk, rr, tid, M, L, all);
+    for (int item = warp; item < n_complete * P.g; item += D8_NW)
+        d8_merge_records<D>(P, complete[item / P.g].records, complete[item / P.g].pair, item % P.g, lane);
 }
 
 // Few pages: a cluster of C CTAs per (sequence, kv head), as decode_cluster_kernel: one launch, the CTAs' states meet in shared
@@ -593,11 +727,10 @@ struct Decode8ClusterSmem {
 };
 
 template <int D>
-__global__ void __launch_bounds__(D8_THREADS, D8_CTAS) decode8_cluster_kernel(const __grid_constant__ Decode8Params P, const int C) {
-    using Smem = Decode8Smem<D>;
+__global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __grid_constant__ Decode8Params P, const int C) {
     constexpr int DG = D / 4;
     extern __shared__ __align__(128) uint8_t d8_smem[];
-    float4* meta = reinterpret_cast<float4*>(d8_smem + Smem::META);
+    __shared__ int ends_with[D8_NW];
     float4* push = reinterpret_cast<float4*>(d8_smem + Decode8ClusterSmem<D>::PUSH);       // [source CTA][column group of this CTA]
     float2* push_ml = reinterpret_cast<float2*>(push + Decode8ClusterSmem<D>::SLOT_F4);    // [source CTA][GP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -607,44 +740,34 @@ __global__ void __launch_bounds__(D8_THREADS, D8_CTAS) decode8_cluster_kernel(co
     const int p_begin = (int)((long long)pages * rank / C), n = (int)((long long)pages * (rank + 1) / C) - p_begin;
     if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before the first push
 
-    const uint32_t ring = smem_u32(d8_smem) + warp * Smem::WARP, scales = smem_u32(d8_smem) + Smem::SCALES + warp * D8_SLOTS * 32;
+    Decode8Ring<D> ring(d8_smem, warp, lane);
     const Decode8Walk start{b, hk, pages, -p_begin};
     Decode8Feed feed;
     feed.init(P, start, warp, n, D8_NW);
-    d8_copy<D>(P, feed, ring, scales, lane);
-    d8_copy<D>(P, feed, ring + Smem::SLOT, scales + 32, lane);
-    Decode8State<D> st;
-    st.load_q(P, b, hk, lane);
-    int slot = 0, free_slot = 2;
-    for (int i = warp; i < n; i += D8_NW) {
-        cp_async_wait<1>();
-        __syncwarp();  // the page is there, and every lane is done with the slot before it
-        d8_copy<D>(P, feed, ring + free_slot * Smem::SLOT, scales + free_slot * 32, lane);
-        st.page(ring + slot * Smem::SLOT, scales + slot * 32, (p_begin + i) * DEC_PT - front, end - front, lane);
-        free_slot = slot;
-        slot = slot == D8_SLOTS - 1 ? 0 : slot + 1;
-    }
-    cp_async_wait<0>();
-    __syncwarp();
-    auto out = [&](int w) { return reinterpret_cast<float*>(d8_smem + w * Smem::WARP); };  // nothing is on its way any more
-    st.reduce();
-    st.store(out(warp), meta + warp * DEC_GP, lane);
+    ring.fill(P, feed, lane);
+    uint32_t* digits = reinterpret_cast<uint32_t*>(d8_smem + ring.spare);  // warp 0's
+    if (warp < DEC_GP * D / 128) d8_digits<D>(P, b, hk, warp, DEC_GP * D / 128, digits, lane);
     __syncthreads();
+    Decode8State<D> st;
+    st.start(digits, lane);
+    __syncthreads();
+    for (int i = warp; i < n; i += D8_NW) ring.page(P, feed, st, (p_begin + i) * DEC_PT - front, end - front, lane);
+    cp_async_wait<0>();
+    __syncwarp();  // nothing is on its way to the slots any more
+    st.reduce();
+    st.store(d8_smem, warp, lane);
+    if (lane == 0) ends_with[warp] = 0;
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster has started
     const int items = P.g * DG, per = (items + C - 1) / C;  // CTA k finishes column groups [k per, (k + 1) per)
-    for (int item = tid; item < items; item += D8_THREADS) {
-        const int rr = item / DG, dg = item % DG;
-        float M, L;
-        float4 acc;
-        d8_merge<D>(meta, out, rr, dg, M, L, acc);
+    d8_merge_warps<D>(d8_smem, ends_with, P.g, [&](int, int, int rr, int dg, float M, float L, float4 acc) {
         if (C == 1) {
             decode_emit(P.res, D, P.g, b, hk, rr, dg, M, L, acc);
         } else {
-            const int to = item / per;
+            const int item = rr * DG + dg, to = item / per;
             st_cluster_f4(map_to_cta(push + rank * per + (item - to * per), (uint32_t)to), acc);
             if (dg < C) st_cluster_f2(map_to_cta(push_ml + rank * DEC_GP + rr, (uint32_t)dg), make_float2(M, L));
         }
-    }
+    });
     if (C == 1) return;
     __syncwarp();
     cluster_sync();  // everything pushed here has arrived

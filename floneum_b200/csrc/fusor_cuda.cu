@@ -1128,6 +1128,7 @@ struct fusor_cuda_kvcache {
     int decode_ctas = 0;              // 0 = automatic grid size
     float* part_o = nullptr;          // [max_slots][DEC_GP][D]
     float* part_ml = nullptr;         // [max_slots][DEC_GP][2]
+    int* done = nullptr;              // 8-bit pages: [max_batch * Hkv], see Decode8Params
     // dense staging for token-granular eviction, grown on demand
     uint8_t* shift_buf = nullptr;
     size_t shift_bytes = 0;
@@ -1171,11 +1172,11 @@ extern "C" int32_t fusor_cuda_kvcache_create_dtype(fusor_cuda_ctx* ctx, int32_t 
     const bool i8 = dtype == FUSOR_CUDA_I8;
     const size_t rows = (size_t)num_pages * num_kv_heads * DEC_PT, pool_bytes = rows * head_dim * (i8 ? 1 : 2);
     void *k_pool = nullptr, *v_pool = nullptr;
-    c->max_grid = (i8 ? D8_CTAS : DEC_CTAS) * ctx->num_sms;
+    c->max_grid = (i8 ? 1 : DEC_CTAS) * ctx->num_sms;
     c->max_slots = max_batch * num_kv_heads + c->max_grid * (i8 ? D8_NW : 1);  // a record per (sequence, kv head) and CTA (8-bit: warp)
     auto alloc = [&](auto** p, size_t bytes) { return ctx->pool.plain(bytes, reinterpret_cast<void**>(p)); };
     bool ok = alloc(&k_pool, pool_bytes) == cudaSuccess && alloc(&v_pool, pool_bytes) == cudaSuccess &&
-              (!i8 || alloc(&c->scales, rows * 2) == cudaSuccess) &&
+              (!i8 || (alloc(&c->scales, rows * 2) == cudaSuccess && alloc(&c->done, (size_t)max_batch * num_kv_heads * 4) == cudaSuccess)) &&
               alloc(&c->d_tables, ((size_t)3 * max_batch + (size_t)max_batch * max_pages_per_seq) * 4) == cudaSuccess &&
               alloc(&c->part_o, (size_t)c->max_slots * DEC_GP * head_dim * 4) == cudaSuccess &&
               alloc(&c->part_ml, (size_t)c->max_slots * DEC_GP * 2 * 4) == cudaSuccess;
@@ -1194,7 +1195,8 @@ extern "C" int32_t fusor_cuda_kvcache_create_dtype(fusor_cuda_ctx* ctx, int32_t 
     }
     if (ok) ok = cudaMemsetAsync(k_pool, 0, pool_bytes, ctx->stream) == cudaSuccess &&
                  cudaMemsetAsync(v_pool, 0, pool_bytes, ctx->stream) == cudaSuccess &&
-                 (!i8 || cudaMemsetAsync(c->scales, 1, rows * 2, ctx->stream) == cudaSuccess) &&  // the byte of a row of zeros
+                 (!i8 || (cudaMemsetAsync(c->scales, 1, rows * 2, ctx->stream) == cudaSuccess &&  // the byte of a row of zeros
+                          cudaMemsetAsync(c->done, 0, (size_t)max_batch * num_kv_heads * 4, ctx->stream) == cudaSuccess)) &&
                  cudaMemsetAsync(c->d_page_table, 0, (size_t)max_batch * max_pages_per_seq * 4, ctx->stream) == cudaSuccess &&
                  cudaMemsetAsync(c->d_end, 0, (size_t)2 * max_batch * 4, ctx->stream) == cudaSuccess;  // ends and fronts
     if (!ok) {
@@ -1232,7 +1234,7 @@ extern "C" int32_t fusor_cuda_kvcache_destroy(fusor_cuda_kvcache* c) {
     if (!c) return FUSOR_CUDA_OK;
     DeviceGuard g(c->ctx->device);
     cudaStreamSynchronize(c->ctx->stream);
-    void* ptrs[] = {c->k_pages, c->v_pages, c->k_codes, c->v_codes, c->scales, c->d_tables, c->part_o, c->part_ml, c->shift_buf};
+    void* ptrs[] = {c->k_pages, c->v_pages, c->k_codes, c->v_codes, c->scales, c->done, c->d_tables, c->part_o, c->part_ml, c->shift_buf};
     for (void* p : ptrs)
         if (p) cudaFree(p);
 
@@ -1854,13 +1856,6 @@ static int32_t launch_combine(fusor_cuda_kvcache* c, const DecodeOutput& res, in
     // record lanes per block: a kv head of a short sequence has one or two records, a 128 K-token sequence ~74
     const long long per_head = longest * grid / std::max<long long>(1, total) + 2;
     const int lanes = per_head <= 4 ? 2 : per_head <= 32 ? 8 : DEC_CL;
-    if (res.mode != 2 && c->k_codes) {
-        const size_t smem = (size_t)(per_head + 3 + D8_MERGE / 32 * c->D) * 4;  // the weights of a head's records, and the warps' sums
-        const auto run = [&](auto kernel) { kernel<<<dim3(res.Hq, B), D8_MERGE, smem, ctx->stream>>>(C); };
-        if (c->D == 128) run(decode8_combine_kernel<128>);
-        else run(decode8_combine_kernel<64>);
-        return launch_check(ctx, "decode8_combine_kernel");
-    }
     if (res.mode != 2) {
         // (the kernel's blocks return at once for heads whose pages all went to one CTA)
         decode_combine_kernel<<<dim3(res.Hq, B), (c->D / 4) * lanes, 0, ctx->stream>>>(C);
@@ -1896,13 +1891,14 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
         }
     }
     // every warp its share, at least a page of it
-    const int grid = c->decode_ctas > 0 ? c->decode_ctas : D8_CTAS * ctx->num_sms;
+    const int grid = c->decode_ctas > 0 ? c->decode_ctas : ctx->num_sms;
     const int shares = (int)std::min<long long>((long long)grid * D8_NW, total);
     if (total > 0) {  // (every chunk empty: only the merge kernel runs and writes empty records)
         const auto run = [&](auto kernel, size_t smem) { kernel<<<(shares + D8_NW - 1) / D8_NW, D8_THREADS, smem, ctx->stream>>>(P, shares); };
         if (c->D == 128) run(decode8_splitkv_kernel<128>, Decode8Smem<128>::bytes);
         else run(decode8_splitkv_kernel<64>, Decode8Smem<64>::bytes);
         TRY(launch_check(ctx, "decode8_splitkv_kernel"));
+        if (P.res.mode != 2) return FUSOR_CUDA_OK;  // it merges its records itself
     }
     return launch_combine(c, P.res, P.B, P.g, shares, total, longest, ex);
 }
@@ -1941,7 +1937,7 @@ static int32_t decode_impl(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* c, const fus
         P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table;
         P.max_pages = c->max_pages; P.num_pages = c->num_pages; P.end = c->d_end; P.front = c->d_front;
         P.B = B; P.Hkv = c->Hkv; P.g = g; P.scale_log2 = scale * 1.4426950408889634f; P.err = ctx->d_err;
-        P.part_o = c->part_o; P.part_ml = c->part_ml;
+        P.part_o = c->part_o; P.part_ml = c->part_ml; P.done = c->done;
         P.res.out = out; P.res.out_dtype = out_dtype; P.res.o_sb = o_sb; P.res.o_sh = o_sh; P.res.Hq = Hq; P.res.mode = mode;
         return decode8_launch(c, P, total, ex);
     }
