@@ -186,6 +186,14 @@ struct Decode8Digits {
     static_assert(WORDS * 4 <= Decode8Smem<D>::SLOT, "they fit a slot");
 };
 
+// The query's lines to L2 while the memory is idle: its loads come behind those of the first pages.
+template <int D>
+__device__ __forceinline__ void d8_prefetch_q(const Decode8Params& P, int b, int hk, int lane) {
+    const int h = lane >> 2, size = P.q_dtype == 0 ? 4 : 2, at = (lane & 3) * 128;
+    if (h >= P.g || at >= D * size) return;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(P.q) + (b * P.q_sb + (long long)(hk * P.g + h) * P.q_sh) * size + at));
+}
+
 // Query heads first, first + step, .. of the group into `digits`, a warp; D = 64: two at a time.  Heads past the last: factor 0, and
 // whatever lies there as digits (whole numbers, so their scores are zeros).
 template <int D>
@@ -608,8 +616,8 @@ __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const D
 // The pages of all (sequence, kv head) pairs, numbered as in decode_splitkv_kernel, are dealt evenly to `shares` warps, each a run of
 // its own: warps meet nobody on the way, copies run on over the ends of sequences, and a pair that a warp has all pages of goes from
 // its registers to the result.  What a warp ends with is merged with the warps of the CTA that end with the same pair, to one
-// record.  Then the CTA adds the pages it had of each pair to a counter, and merges the records of those that are complete with
-// it: no second launch, and no order of arrival in a result.
+// record, or to the result when the CTA has all of it.  Of the pairs that it shares with other CTAs it adds the pages it had to a counter,
+// and merges the records of those that are complete with it: no second launch, and no order of arrival in a result.
 template <int D>
 __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __grid_constant__ Decode8Params P, const int shares) {
     using Smem = Decode8Smem<D>;
@@ -651,6 +659,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     Decode8Ring<D> ring(d8_smem, warp, lane);
     Decode8Feed feed;
     feed.init(P, w, 0, n, 1);
+    if (n > 0) d8_prefetch_q<D>(P, w.b, w.hk, lane);
     ring.fill(P, feed, lane);
 
     if (P.res.mode == 1)  // sequences without pages: empty records
@@ -688,8 +697,23 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
         if (i >= n) break;
     }
     if (lane == 0) ends_with[warp] = open;
+    const int cta_first = deal.bound(cta0), cta_end = deal.bound(cta0 + D8_NW);
+    const auto inside = [&](int4 part) { return part.y >= cta_first && part.y + part.w <= cta_end && P.res.mode != 2; };  // all its pages are this CTA's
     d8_merge_warps<D>(d8_smem, ends_with, P.g, [&](int w0, int size, int rr, int dg, float M, float L, float4 acc) {
-        const long long rec = ((long long)ends_with[w0] + cta0 + w0) * DEC_GP + rr;
+        const int pair = ends_with[w0];
+        const long long rec = ((long long)pair + cta0 + w0) * DEC_GP + rr;
+        if (inside(parts[2 * w0 + 1])) {
+            if (w0 + size < D8_NW && parts[2 * (w0 + size)].z > 0 && parts[2 * (w0 + size)].x == pair) {  // and the record of the warp that it ends inside of
+                const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + (rec + size * DEC_GP) * 2);
+                const float4 o = *reinterpret_cast<const float4*>(P.part_o + (rec + size * DEC_GP) * D + dg * 4);
+                const float top = fmaxf(M, ml.x), a0 = L == 0.0f ? 0.0f : fast_exp2(M - top), a1 = ml.y == 0.0f ? 0.0f : fast_exp2(ml.x - top);
+                acc.x = acc.x * a0 + o.x * a1; acc.y = acc.y * a0 + o.y * a1; acc.z = acc.z * a0 + o.z * a1; acc.w = acc.w * a0 + o.w * a1;
+                L = L * a0 + ml.y * a1;
+                M = top;
+            }
+            decode_emit(P.res, D, P.g, pair / P.Hkv, pair % P.Hkv, rr, dg, M, L, acc);
+            return;
+        }
         *reinterpret_cast<float4*>(P.part_o + rec * D + dg * 4) = acc;
         if (dg == 0) {
             *reinterpret_cast<float2*>(P.part_ml + rec * 2) = make_float2(M, L);
@@ -702,7 +726,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     // ---- the pairs that are complete with this CTA's pages
     __threadfence();
     __syncthreads();  // this CTA's records can be seen everywhere
-    if (tid < 2 * D8_NW && parts[tid].z > 0) {
+    if (tid < 2 * D8_NW && parts[tid].z > 0 && !inside(parts[tid])) {
         const int4 part = parts[tid];
         const int pair = part.x, before = atomicAdd(P.done + pair, part.z);
         const Decode8Records R(deal, part.y, part.w);
