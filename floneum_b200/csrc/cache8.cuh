@@ -73,7 +73,190 @@ __device__ __forceinline__ int place_row(const PlaceParams& P, int b, int t, int
     return 0;
 }
 
-// One warp per row of q, k or v.
+// ---------------------------------------------------------------------------------------------------------------
+// The vector form, for D a multiple of 16, tensors of one type and 16-byte aligned rows: a thread takes 16 elements of a row, 8 pairs with
+// their cos / sin values, and walks heads with them.  HBM-bound: several heads' loads are issued together, one thread per item.  The
+// D / 16 threads of a row are neighbours in a warp and find its largest element by shuffles.
+template <int T>
+struct PlaceType {
+    static constexpr int ES = T == 0 ? 4 : 2, U4 = ES / 2;  // bytes of an element; 16-byte vectors of 8 of them
+};
+
+// Eight elements from `base + at`, in flight until place_floats
+template <int T>
+__device__ __forceinline__ void place_fetch(const void* base, long long at, uint4 (&raw)[PlaceType<T>::U4]) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at * PlaceType<T>::ES);
+#pragma unroll
+    for (int j = 0; j < PlaceType<T>::U4; ++j) raw[j] = __ldcs(p + j);
+}
+template <int T>
+__device__ __forceinline__ void place_floats(const uint4 (&raw)[PlaceType<T>::U4], float (&f)[8]) {
+    if (T == 0) {
+        const uint4 a = raw[0], b = raw[PlaceType<T>::U4 - 1];
+        f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+        f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
+    } else {
+        rope_unpack16<T == 2>(raw[0], f);
+    }
+}
+
+// cos and sin of pairs i0 .. i0 + 7 of token t of sequence b
+__device__ __forceinline__ void place_angles(const PlaceParams& P, int b, int t, int i0, float (&c)[8], float (&s)[8]) {
+    const int half = P.D >> 1;
+    bool one = !P.pos;  // one axis for all eight: vector loads
+    if (!one) {
+        const uint2 axes = *reinterpret_cast<const uint2*>(P.axis + i0);
+        one = axes.x == axes.y && axes.x == (axes.x & 0xffu) * 0x01010101u;
+    }
+    if (one) {
+        const long long at = (long long)place_row(P, b, t, i0) * half + i0;
+        rope_load8(P.cos_t, 0, at, c);
+        rope_load8(P.sin_t, 0, at, s);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const long long at = (long long)place_row(P, b, t, i0 + j) * half + i0 + j;
+        c[j] = __ldg(P.cos_t + at);
+        s[j] = __ldg(P.sin_t + at);
+    }
+}
+
+// 16 elements of a row, this thread's, as codes in cv (the first eight, the others) and the row's byte.  GROUP threads share the row.
+// x / 2^e + 1.5 * 2^23 rounds to the code, ties to even, and has it in its low byte.
+template <int GROUP>
+__device__ __forceinline__ int place_codes(float (&a)[8], float (&z)[8], uint2 (&cv)[2]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, max(abs_bits(a[j]), abs_bits(z[j])));
+#pragma unroll
+    for (int x = 1; x < GROUP; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const int byte = row8_byte(__uint_as_float(top));
+    const float inverse = row8_inverse(min(byte, kRowTop));
+    if (byte >= kRowTop) {  // seldom: values beyond the last step end at 127, rows that are not finite have codes of 0
+        const float most = byte == kRowTop ? 127.0f * row8_step(kRowTop) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            a[j] = fmaxf(fminf(a[j], most), -most);
+            z[j] = fmaxf(fminf(z[j], most), -most);
+        }
+    }
+    constexpr float MAGIC = 12582912.0f;
+    const auto pack = [&](const float* x) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __float_as_uint(fmaf(x[j], inverse, MAGIC));
+        return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    };
+    cv[0] = make_uint2(pack(a), pack(a + 4));
+    cv[1] = make_uint2(pack(z), pack(z + 4));
+    return byte;
+}
+
+// PAGES: 0 q alone, 1 bf16 pages, 2 8-bit pages.  ROT: 0 none (no q), 1 halves, 2 adjacent pairs.  T: type of all tensors.  The first
+// q_blocks blocks do q, the others k and v.
+template <int PAGES, int ROT, int T, int D>
+__global__ void __launch_bounds__(256) place_vec_kernel(const __grid_constant__ PlaceParams P, const unsigned q_blocks, const unsigned per_thread) {
+    if (PAGES) P.lens.publish();
+    constexpr int U4 = PlaceType<T>::U4, U = T == 0 ? 2 : 4, V = T == 0 ? 1 : 2;  // heads of q, and of k and v, whose loads are in flight
+    const int d = D ? D : P.D, half = d >> 1;
+    const unsigned chunks = (unsigned)d >> 4;
+    const bool is_q = blockIdx.x < q_blocks;
+    const unsigned heads = (unsigned)(is_q ? P.Hq : P.Hkv), per = is_q ? per_thread : max(1u, per_thread / 2), groups = (heads + per - 1) / per;
+    const unsigned long long total = (unsigned long long)P.B * groups * P.n * chunks;
+    unsigned long long idx = (unsigned long long)(is_q ? blockIdx.x : blockIdx.x - q_blocks) * blockDim.x + threadIdx.x;
+    const bool live = idx < total;  // (the others stay for the shuffles)
+    if (!live) idx = total - 1;
+    const unsigned ch = (unsigned)(idx % chunks);
+    const unsigned long long r = idx / chunks;
+    const unsigned t = (unsigned)(r % (unsigned)P.n), bg = (unsigned)(r / (unsigned)P.n);
+    const unsigned b = bg / groups, h_begin = bg % groups * per, h_end = live ? min(heads, h_begin + per) : 0;
+    const int i0 = (int)ch * 8;
+    const int offa = ROT == 1 ? i0 : 2 * i0, offz = ROT == 1 ? i0 + half : 2 * i0 + 8;
+    float c[8], s[8];
+    if (is_q) {
+        const long long src = b * P.qs[0] + t * P.qs[2], dst = b * P.qos[0] + t * P.qos[2];
+        for (unsigned h0 = h_begin; h0 < h_end; h0 += U) {
+            uint4 a[U][U4], z[U][U4];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (h0 + u < h_end) {
+                    place_fetch<T>(P.q, src + (h0 + u) * P.qs[1] + offa, a[u]);
+                    place_fetch<T>(P.q, src + (h0 + u) * P.qs[1] + offz, z[u]);
+                }
+            if (h0 == h_begin) place_angles(P, (int)b, (int)t, i0, c, s);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (h0 + u < h_end) {
+                    float xa[8], xz[8];
+                    place_floats<T>(a[u], xa);
+                    place_floats<T>(z[u], xz);
+                    rope_rotate8<ROT == 2>(xa, xz, c, s);
+                    rope_store8(P.q_out, T, dst + (h0 + u) * P.qos[1] + offa, xa);
+                    rope_store8(P.q_out, T, dst + (h0 + u) * P.qos[1] + offz, xz);
+                }
+        }
+        return;
+    }
+    if (PAGES == 0) return;
+    const int at = P.lens.before((int)b) + (int)t;
+    const int page = P.page_table[(long long)b * P.max_pages + at / DEC_PT];
+    const long long ksrc = b * P.ks[0] + t * P.ks[2], vsrc = b * P.vs[0] + t * P.vs[2];
+    for (unsigned k = 0; k < per; k += V) {
+        const unsigned h0 = h_begin + k;
+        uint4 a[V][U4], z[V][U4], va[V][U4], vz[V][U4];
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+            if (h0 + u < h_end) {
+                place_fetch<T>(P.k_new, ksrc + (h0 + u) * P.ks[1] + offa, a[u]);
+                place_fetch<T>(P.k_new, ksrc + (h0 + u) * P.ks[1] + offz, z[u]);
+                place_fetch<T>(P.v_new, vsrc + (h0 + u) * P.vs[1] + 2 * i0, va[u]);
+                place_fetch<T>(P.v_new, vsrc + (h0 + u) * P.vs[1] + 2 * i0 + 8, vz[u]);
+            }
+        if (ROT && k == 0) place_angles(P, (int)b, (int)t, i0, c, s);
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            float xa[8] = {}, xz[8] = {}, ya[8] = {}, yz[8] = {};
+            if (h0 + u < h_end) {
+                place_floats<T>(a[u], xa);
+                place_floats<T>(z[u], xz);
+                place_floats<T>(va[u], ya);
+                place_floats<T>(vz[u], yz);
+                if (ROT) rope_rotate8<ROT == 2>(xa, xz, c, s);
+            }
+            const long long tile = (long long)page * P.Hkv + (h0 + u), dst = (tile * DEC_PT + at % DEC_PT) * d;
+            if (PAGES == 1) {
+                if (h0 + u < h_end) {
+                    rope_store8(P.k_pages, 1, dst + offa, xa);
+                    rope_store8(P.k_pages, 1, dst + offz, xz);
+                    rope_store8(P.v_pages, 1, dst + 2 * i0, ya);
+                    rope_store8(P.v_pages, 1, dst + 2 * i0 + 8, yz);
+                }
+            } else {
+                constexpr int GROUP = D ? D / 16 : 1;
+                uint2 kc[2], vc[2];
+                const int kb = place_codes<GROUP>(xa, xz, kc), vb = place_codes<GROUP>(ya, yz, vc);
+                if (h0 + u < h_end) {
+                    uint8_t* kp = static_cast<uint8_t*>(P.k_pages) + dst;
+                    if (ROT == 1) {
+                        *reinterpret_cast<uint2*>(kp + offa) = kc[0];
+                        *reinterpret_cast<uint2*>(kp + offz) = kc[1];
+                    } else {
+                        *reinterpret_cast<uint4*>(kp + 2 * i0) = make_uint4(kc[0].x, kc[0].y, kc[1].x, kc[1].y);
+                    }
+                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(P.v_pages) + dst + 2 * i0) = make_uint4(vc[0].x, vc[0].y, vc[1].x, vc[1].y);
+                    if (ch == 0) {
+                        uint8_t* scale = P.scales + tile * 2 * DEC_PT + at % DEC_PT;
+                        scale[0] = (uint8_t)kb;
+                        scale[DEC_PT] = (uint8_t)vb;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// What the vector form does not take: one warp per row of q, k or v.
 __global__ void __launch_bounds__(256) place_rows_kernel(const __grid_constant__ PlaceParams P) {
     if (P.pages) P.lens.publish();
     const int lane = threadIdx.x & 31, half = P.D >> 1;
@@ -136,23 +319,53 @@ struct Gather8Params {
     int max_pages, Hkv, D, len, B;
 };
 
-__global__ void __launch_bounds__(256) kvcache8_gather_kernel(const __grid_constant__ Gather8Params P) {
-    const long long total = (long long)P.B * P.Hkv * P.len * P.D;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const int d = (int)(i % P.D);
-        const int t = (int)((i / P.D) % P.len);
-        const int hk = (int)((i / ((long long)P.D * P.len)) % P.Hkv);
-        const int b = (int)(i / ((long long)P.D * P.len * P.Hkv));
-        float kf = 0.0f, vf = 0.0f;
-        const int at = P.front[b] + t;
-        if (at < P.end[b]) {
-            const long long tile = (long long)P.page_table[(long long)b * P.max_pages + at / DEC_PT] * P.Hkv + hk;
-            const long long src = (tile * DEC_PT + at % DEC_PT) * P.D + d;
-            kf = row8_step(P.scales[tile * 2 * DEC_PT + at % DEC_PT]) * (float)P.k_codes[src];
-            vf = row8_step(P.scales[(tile * 2 + 1) * DEC_PT + at % DEC_PT]) * (float)P.v_codes[src];
+// Four codes times a step: the byte with its sign bit flipped under the exponent of 2^23, which is then taken off.  Exact.
+__device__ __forceinline__ void row8_values(uint32_t codes, float step, float (&f)[4]) {
+    const uint32_t w = codes ^ 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)) - 8388736.0f) * step;
+}
+
+// A thread takes 16 codes of a row of K and of V.  vec: rows of the results start on multiples of 16 bytes.  blockIdx.y: (sequence, kv head).
+__global__ void __launch_bounds__(256) kvcache8_gather_kernel(const __grid_constant__ Gather8Params P, const int vec) {
+    const int chunks = P.D / 16;
+    for (int pair = blockIdx.y; pair < P.B * P.Hkv; pair += gridDim.y) {
+        const int b = pair / P.Hkv, hk = pair % P.Hkv, front = __ldg(P.front + b), end = __ldg(P.end + b);
+        for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < (long long)P.len * chunks; i += (long long)gridDim.x * blockDim.x) {
+            const int c = (int)(i % chunks) * 16, t = (int)(i / chunks), at = front + t;
+            uint4 code[2] = {};
+            float step[2] = {0.0f, 0.0f};
+            if (at < end) {
+                const long long tile = (long long)P.page_table[(long long)b * P.max_pages + at / DEC_PT] * P.Hkv + hk;
+                const long long src = (tile * DEC_PT + at % DEC_PT) * P.D + c;
+                code[0] = __ldg(reinterpret_cast<const uint4*>(P.k_codes + src));
+                code[1] = __ldg(reinterpret_cast<const uint4*>(P.v_codes + src));
+                const uint8_t* scale = P.scales + tile * 2 * DEC_PT + at % DEC_PT;
+                step[0] = row8_step(__ldg(scale));
+                step[1] = row8_step(__ldg(scale + DEC_PT));
+            }
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                void* out = which ? P.v_out : P.k_out;
+                const int dtype = which ? P.v_dtype : P.k_dtype;
+                const long long* st = which ? P.vs : P.ks;
+                const long long dst = b * st[0] + hk * st[1] + t * st[2] + c;
+                const uint32_t w[4] = {code[which].x, code[which].y, code[which].z, code[which].w};
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    float lo[4], hi[4];
+                    row8_values(w[j], step[which], lo);
+                    row8_values(w[j + 1], step[which], hi);
+                    const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    if (vec) {
+                        rope_store8(out, dtype, dst + 4 * j, f);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) st_from_float(out, dtype, dst + 4 * j + e, f[e]);
+                    }
+                }
+            }
         }
-        st_from_float(P.k_out, P.k_dtype, b * P.ks[0] + hk * P.ks[1] + t * P.ks[2] + d, kf);
-        st_from_float(P.v_out, P.v_dtype, b * P.vs[0] + hk * P.vs[1] + t * P.vs[2] + d, vf);
     }
 }
 

@@ -1338,8 +1338,39 @@ static int32_t kv_reserve(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new
     return FUSOR_CUDA_OK;
 }
 
-// Rows through place_rows_kernel: rotated (where P has tables), to either cache (where P has pages).
+static bool rope_vec_ok(const void* p, int dtype, const long long* stride);
+
+template <int PAGES, int ROT, int D>
+static void place_vec_run(fusor_cuda_ctx* ctx, const PlaceParams& P, int type, unsigned blocks, unsigned q_blocks, unsigned per) {
+    const auto run = [&](auto kernel) { kernel<<<blocks, 256, 0, ctx->stream>>>(P, q_blocks, per); };
+    if (type == FUSOR_CUDA_F32) run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_F32, D>);
+    else if (type == FUSOR_CUDA_BF16) run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_BF16, D>);
+    else run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_F16, D>);
+}
+
+// Rows to their places: rotated (where P has tables), to either cache (where P has pages).
 static int32_t place_launch(fusor_cuda_ctx* ctx, const PlaceParams& P) {
+    const int type = P.Hq ? P.q_dtype : P.k_dtype;
+    bool vec = P.D % 16 == 0 && reinterpret_cast<uintptr_t>(P.cos_t) % 16 == 0 && reinterpret_cast<uintptr_t>(P.sin_t) % 16 == 0;
+    if (P.Hq) vec = vec && P.qo_dtype == type && rope_vec_ok(P.q, type, P.qs) && rope_vec_ok(P.q_out, type, P.qos);
+    if (P.pages) vec = vec && P.k_dtype == type && P.v_dtype == type && rope_vec_ok(P.k_new, type, P.ks) && rope_vec_ok(P.v_new, type, P.vs);
+    if (vec) {
+        // eight query heads (half as many kv heads) a thread, halved while fewer than 1024 threads per SM would be left, down to two
+        const long long items = (long long)P.B * P.n * (P.D / 16);
+        const auto q_threads = [&](int per) { return items * ((P.Hq + per - 1) / per); };
+        const auto kv_threads = [&](int per) { return P.pages ? items * ((P.Hkv + per / 2 - 1) / (per / 2)) : 0; };
+        int per = 8;
+        while (per > 2 && q_threads(per) + kv_threads(per) < 1024ll * ctx->num_sms) per /= 2;
+        const long long q_blocks = (q_threads(per) + 255) / 256, blocks = q_blocks + (kv_threads(per) + 255) / 256;
+        if (blocks <= 0x7fffffffLL) {
+            const auto go = [&](auto run) { run(ctx, P, type, (unsigned)blocks, (unsigned)q_blocks, (unsigned)per); };
+            if (P.pages == 0) go(P.interleaved ? place_vec_run<0, 2, 0> : place_vec_run<0, 1, 0>);
+            else if (P.pages == 1) go(P.interleaved ? place_vec_run<1, 2, 0> : place_vec_run<1, 1, 0>);
+            else if (P.D == 128) go(!P.cos_t ? place_vec_run<2, 0, 128> : P.interleaved ? place_vec_run<2, 2, 128> : place_vec_run<2, 1, 128>);
+            else go(!P.cos_t ? place_vec_run<2, 0, 64> : P.interleaved ? place_vec_run<2, 2, 64> : place_vec_run<2, 1, 64>);
+            return launch_check(ctx, "place_vec_kernel");
+        }
+    }
     const long long rows = (long long)P.B * P.n * (P.Hq + (P.pages ? 2 * P.Hkv : 0));
     const int blocks = (int)std::max<long long>(1, std::min<long long>((rows + 7) / 8, (long long)ctx->num_sms * 16));
     place_rows_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
@@ -1690,8 +1721,11 @@ extern "C" int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* c, const fusor_
         for (int i = 0; i < 3; ++i) { P.ks[i] = k_out->stride[i]; P.vs[i] = v_out->stride[i]; }
         P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
         P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.D = c->D; P.len = longest; P.B = c->active_B;
-        const int blocks = (int)std::max<long long>(1, std::min<long long>((total + 255) / 256, (long long)ctx->num_sms * 8));
-        kvcache8_gather_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+        if (total == 0) return FUSOR_CUDA_OK;
+        const bool vec = rope_vec_ok(P.k_out, P.k_dtype, P.ks) && rope_vec_ok(P.v_out, P.v_dtype, P.vs);
+        const long long threads = (long long)longest * (c->D / 16);
+        const dim3 grid((unsigned)std::min<long long>((threads + 255) / 256, 1 << 20), (unsigned)std::min(P.B * P.Hkv, 65535));
+        kvcache8_gather_kernel<<<grid, (unsigned)std::min<long long>(256, (threads + 31) / 32 * 32), 0, ctx->stream>>>(P, vec ? 1 : 0);
         return launch_check(ctx, "kvcache8_gather_kernel");
     }
     GatherParams P;
