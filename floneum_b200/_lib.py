@@ -32,7 +32,7 @@ class Tensor2(ctypes.Structure):
 
 class RopePositions(ctypes.Structure):
     _fields_ = [("ids", c_void_p), ("axis_stride", c_int64), ("batch_stride", c_int64), ("n_axes", c_int32), ("_pad", c_int32),
-                ("axis_of_pair", c_void_p)]
+                ("axis_of_pair", c_char_p)]
 
 
 class FusorCudaError(RuntimeError):
@@ -94,11 +94,12 @@ SIGNATURES = {
     "fusor_cuda_rope": (c_int32, [c_void_p, _T4, c_void_p, c_void_p, c_int32, c_int32, c_int32, _T4]),
     "fusor_cuda_kvcache_rope_append": (c_int32, [c_void_p, _T4, _T4, _T4, c_void_p, c_void_p, c_int32, c_int32, c_int32, _T4]),
     "fusor_cuda_rope_axes": (c_int32, [c_void_p, _T4, c_void_p, c_void_p, c_int32, _RP, c_int32, _T4]),
+    "fusor_cuda_rope_axes_qk": (c_int32, [c_void_p, _T4, _T4, c_void_p, c_void_p, c_int32, _RP, c_int32, _T4, _T4]),
     "fusor_cuda_kvcache_rope_axes_append": (c_int32, [c_void_p, _T4, _T4, _T4, c_void_p, c_void_p, c_int32, _RP, c_int32, _T4]),
     "fusor_cuda_kvcache_truncate_front": (c_int32, [c_void_p, c_int32, c_int32]),
     "fusor_cuda_kvcache_drop_front": (c_int32, [c_void_p, c_int32, c_int32]),
     "fusor_cuda_kvcache_seq_len": (c_int32, [c_void_p, c_int32, POINTER(c_int32)]),
-    "fusor_cuda_kvcache_set_page_table": (c_int32, [c_void_p, POINTER(c_int32), POINTER(c_int32), c_int32]),
+    "fusor_cuda_kvcache_set_page_table": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32]),
     "fusor_cuda_kvcache_write_pages": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "fusor_cuda_kvcache_read_pages": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "fusor_cuda_kvcache_pools": (c_int32, [c_void_p, POINTER(c_void_p), POINTER(c_void_p)]),

@@ -158,7 +158,7 @@ class PagedKvCache:
         cq, ck, cv, co = q._c4(), k_new._c4(), v_new._c4(), q_out._c4()
         if positions is not None:
             from .rope import _positions
-            pos, keep = _positions(positions, axes, q.shape()[0], q.shape()[2], self.head_dim)
+            pos = _positions(positions, axes, q.shape()[0], q.shape()[2], self.head_dim)
             self._ck(self._L.fusor_cuda_kvcache_rope_axes_append(self._h, ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv),
                                                                  cos.ptr, sin.ptr, cos.shape()[0], ctypes.byref(pos),
                                                                  int(bool(interleaved)), ctypes.byref(co)))
@@ -184,9 +184,7 @@ class PagedKvCache:
         pt = np.ascontiguousarray(page_table, dtype=np.int32)
         kl = np.ascontiguousarray(kv_len, dtype=np.int32)
         assert pt.ndim == 2 and pt.shape[1] == self.max_pages_per_seq and kl.shape == (pt.shape[0],)
-        i32p = ctypes.POINTER(ctypes.c_int32)
-        self._ck(self._L.fusor_cuda_kvcache_set_page_table(self._h, pt.ctypes.data_as(i32p), kl.ctypes.data_as(i32p),
-                                                           pt.shape[0]))
+        self._ck(self._L.fusor_cuda_kvcache_set_page_table(self._h, pt.ctypes.data, kl.ctypes.data, pt.shape[0]))
 
     def write_pages(self, first_page: int, k_bits: np.ndarray, v_bits: np.ndarray):
         """k_bits, v_bits: uint16 bf16 bit patterns [n_pages, Hkv, page_tokens, D]; int8 codes for an 8-bit cache, whose

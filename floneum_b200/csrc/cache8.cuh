@@ -11,6 +11,8 @@
 // its places (byte 255).
 //   k_codes, v_codes : int8 [num_pages][Hkv][16][D],   scales : uint8 [num_pages][Hkv][2][16]  (K, V)
 #pragma once
+#include <type_traits>
+
 #include "decode_splitkv.cuh"
 #include "rope_append.cuh"
 
@@ -35,6 +37,7 @@ __device__ __forceinline__ int row8_code(float x, float inverse) { return max(-1
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // Rows to place: q [B][Hq][n][D] -> q_out, k_new and v_new [B][Hkv][n][D] -> pages, q and k rotated on the way when there are tables.
+// Without pages k_new (where Hkv > 0) goes to a dense tensor too: k_pages, of type v_dtype and strides vs.
 struct PlaceParams {
     const void* q;  // with Hq = 0: none
     void* q_out;
@@ -122,19 +125,26 @@ __device__ __forceinline__ void place_angles(const PlaceParams& P, int b, int t,
     }
 }
 
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 16 elements of a row, this thread's, as codes in cv (the first eight, the others) and the row's byte.  GROUP threads share the row.
 // x / 2^e + 1.5 * 2^23 rounds to the code, ties to even, and has it in its low byte.
 template <int GROUP>
 __device__ __forceinline__ int place_codes(float (&a)[8], float (&z)[8], uint2 (&cv)[2]) {
-    uint32_t top = 0;
+    float most = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, max(abs_bits(a[j]), abs_bits(z[j])));
+    for (int j = 0; j < 8; ++j) most = fmax3_nan(most, fabsf(a[j]), fabsf(z[j]));
+    uint32_t top = __float_as_uint(most);
 #pragma unroll
     for (int x = 1; x < GROUP; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
     const int byte = row8_byte(__uint_as_float(top));
     const float inverse = row8_inverse(min(byte, kRowTop));
     if (byte >= kRowTop) {  // seldom: values beyond the last step end at 127, rows that are not finite have codes of 0
-        const float most = byte == kRowTop ? 127.0f * row8_step(kRowTop) : 0.0f;
+        most = byte == kRowTop ? 127.0f * row8_step(kRowTop) : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             a[j] = fmaxf(fminf(a[j], most), -most);
@@ -153,36 +163,39 @@ __device__ __forceinline__ int place_codes(float (&a)[8], float (&z)[8], uint2 (
     return byte;
 }
 
-// PAGES: 0 q alone, 1 bf16 pages, 2 8-bit pages.  ROT: 0 none (no q), 1 halves, 2 adjacent pairs.  T: type of all tensors.  The first
-// q_blocks blocks do q, the others k and v.
+// PAGES: 0 q alone, 1 bf16 pages, 2 8-bit pages.  ROT: 0 none (no q), 1 halves, 2 adjacent pairs.  T: type of all tensors.  blockIdx.y:
+// sequence, and a group of query heads or, from q_groups on, of kv heads.
 template <int PAGES, int ROT, int T, int D>
-__global__ void __launch_bounds__(256) place_vec_kernel(const __grid_constant__ PlaceParams P, const unsigned q_blocks, const unsigned per_thread) {
-    if (PAGES) P.lens.publish();
-    constexpr int U4 = PlaceType<T>::U4, U = T == 0 ? 2 : 4, V = T == 0 ? 1 : 2;  // heads of q, and of k and v, whose loads are in flight
+__global__ void __launch_bounds__(256, 3) place_vec_kernel(const __grid_constant__ PlaceParams P, const unsigned q_groups, const unsigned per_thread) {
+    if (PAGES && blockIdx.y == 0) P.lens.publish();
+    constexpr int U4 = PlaceType<T>::U4, U = T == 0 ? 1 : 2;  // query heads whose loads are in flight (of k and v: one head's)
     const int d = D ? D : P.D, half = d >> 1;
     const unsigned chunks = (unsigned)d >> 4;
-    const bool is_q = blockIdx.x < q_blocks;
-    const unsigned heads = (unsigned)(is_q ? P.Hq : P.Hkv), per = is_q ? per_thread : max(1u, per_thread / 2), groups = (heads + per - 1) / per;
-    const unsigned long long total = (unsigned long long)P.B * groups * P.n * chunks;
-    unsigned long long idx = (unsigned long long)(is_q ? blockIdx.x : blockIdx.x - q_blocks) * blockDim.x + threadIdx.x;
-    const bool live = idx < total;  // (the others stay for the shuffles)
-    if (!live) idx = total - 1;
-    const unsigned ch = (unsigned)(idx % chunks);
-    const unsigned long long r = idx / chunks;
-    const unsigned t = (unsigned)(r % (unsigned)P.n), bg = (unsigned)(r / (unsigned)P.n);
-    const unsigned b = bg / groups, h_begin = bg % groups * per, h_end = live ? min(heads, h_begin + per) : 0;
+    const unsigned kv_groups = gridDim.y / (unsigned)P.B - q_groups;
+    const unsigned b = blockIdx.y / (q_groups + kv_groups), group = blockIdx.y % (q_groups + kv_groups);
+    const bool is_q = group < q_groups;
+    const bool dense = is_q || PAGES == 0;  // (k beside q)
+    const unsigned heads = (unsigned)(is_q ? P.Hq : P.Hkv), per = dense ? per_thread : max(1u, per_thread / 2);
+    unsigned idx = blockIdx.x * blockDim.x + threadIdx.x;
+    const bool live = idx < (unsigned)P.n * chunks;  // (the others stay for the shuffles)
+    if (!live) idx = (unsigned)P.n * chunks - 1;
+    const unsigned ch = idx % chunks, t = idx / chunks;
+    const unsigned h_begin = (is_q ? group : group - q_groups) * per, h_end = live ? min(heads, h_begin + per) : 0;
     const int i0 = (int)ch * 8;
     const int offa = ROT == 1 ? i0 : 2 * i0, offz = ROT == 1 ? i0 + half : 2 * i0 + 8;
     float c[8], s[8];
-    if (is_q) {
-        const long long src = b * P.qs[0] + t * P.qs[2], dst = b * P.qos[0] + t * P.qos[2];
+    if (dense) {
+        const void* x = is_q ? P.q : P.k_new;
+        void* out = is_q ? P.q_out : P.k_pages;
+        const long long *xs = is_q ? P.qs : P.ks, *os = is_q ? P.qos : P.vs;
+        const long long src = b * xs[0] + t * xs[2], dst = b * os[0] + t * os[2];
         for (unsigned h0 = h_begin; h0 < h_end; h0 += U) {
             uint4 a[U][U4], z[U][U4];
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (h0 + u < h_end) {
-                    place_fetch<T>(P.q, src + (h0 + u) * P.qs[1] + offa, a[u]);
-                    place_fetch<T>(P.q, src + (h0 + u) * P.qs[1] + offz, z[u]);
+                    place_fetch<T>(x, src + (h0 + u) * xs[1] + offa, a[u]);
+                    place_fetch<T>(x, src + (h0 + u) * xs[1] + offz, z[u]);
                 }
             if (h0 == h_begin) place_angles(P, (int)b, (int)t, i0, c, s);
 #pragma unroll
@@ -192,8 +205,8 @@ __global__ void __launch_bounds__(256) place_vec_kernel(const __grid_constant__ 
                     place_floats<T>(a[u], xa);
                     place_floats<T>(z[u], xz);
                     rope_rotate8<ROT == 2>(xa, xz, c, s);
-                    rope_store8(P.q_out, T, dst + (h0 + u) * P.qos[1] + offa, xa);
-                    rope_store8(P.q_out, T, dst + (h0 + u) * P.qos[1] + offz, xz);
+                    rope_store8(out, T, dst + (h0 + u) * os[1] + offa, xa);
+                    rope_store8(out, T, dst + (h0 + u) * os[1] + offz, xz);
                 }
         }
         return;
@@ -202,54 +215,50 @@ __global__ void __launch_bounds__(256) place_vec_kernel(const __grid_constant__ 
     const int at = P.lens.before((int)b) + (int)t;
     const int page = P.page_table[(long long)b * P.max_pages + at / DEC_PT];
     const long long ksrc = b * P.ks[0] + t * P.ks[2], vsrc = b * P.vs[0] + t * P.vs[2];
-    for (unsigned k = 0; k < per; k += V) {
-        const unsigned h0 = h_begin + k;
-        uint4 a[V][U4], z[V][U4], va[V][U4], vz[V][U4];
-#pragma unroll
-        for (int u = 0; u < V; ++u)
-            if (h0 + u < h_end) {
-                place_fetch<T>(P.k_new, ksrc + (h0 + u) * P.ks[1] + offa, a[u]);
-                place_fetch<T>(P.k_new, ksrc + (h0 + u) * P.ks[1] + offz, z[u]);
-                place_fetch<T>(P.v_new, vsrc + (h0 + u) * P.vs[1] + 2 * i0, va[u]);
-                place_fetch<T>(P.v_new, vsrc + (h0 + u) * P.vs[1] + 2 * i0 + 8, vz[u]);
-            }
+    for (unsigned k = 0; k < per; ++k) {
+        const unsigned h = h_begin + k;
+        const bool here = h < h_end;
+        uint4 a[U4], z[U4], va[U4], vz[U4];
+        if (here) {
+            place_fetch<T>(P.k_new, ksrc + h * P.ks[1] + offa, a);
+            place_fetch<T>(P.k_new, ksrc + h * P.ks[1] + offz, z);
+            place_fetch<T>(P.v_new, vsrc + h * P.vs[1] + 2 * i0, va);
+            place_fetch<T>(P.v_new, vsrc + h * P.vs[1] + 2 * i0 + 8, vz);
+        }
         if (ROT && k == 0) place_angles(P, (int)b, (int)t, i0, c, s);
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-            float xa[8] = {}, xz[8] = {}, ya[8] = {}, yz[8] = {};
-            if (h0 + u < h_end) {
-                place_floats<T>(a[u], xa);
-                place_floats<T>(z[u], xz);
-                place_floats<T>(va[u], ya);
-                place_floats<T>(vz[u], yz);
-                if (ROT) rope_rotate8<ROT == 2>(xa, xz, c, s);
+        float xa[8] = {}, xz[8] = {}, ya[8] = {}, yz[8] = {};
+        if (here) {
+            place_floats<T>(a, xa);
+            place_floats<T>(z, xz);
+            place_floats<T>(va, ya);
+            place_floats<T>(vz, yz);
+            if (ROT) rope_rotate8<ROT == 2>(xa, xz, c, s);
+        }
+        const long long tile = (long long)page * P.Hkv + h, dst = (tile * DEC_PT + at % DEC_PT) * d;
+        if (PAGES == 1) {
+            if (here) {
+                rope_store8(P.k_pages, 1, dst + offa, xa);
+                rope_store8(P.k_pages, 1, dst + offz, xz);
+                rope_store8(P.v_pages, 1, dst + 2 * i0, ya);
+                rope_store8(P.v_pages, 1, dst + 2 * i0 + 8, yz);
             }
-            const long long tile = (long long)page * P.Hkv + (h0 + u), dst = (tile * DEC_PT + at % DEC_PT) * d;
-            if (PAGES == 1) {
-                if (h0 + u < h_end) {
-                    rope_store8(P.k_pages, 1, dst + offa, xa);
-                    rope_store8(P.k_pages, 1, dst + offz, xz);
-                    rope_store8(P.v_pages, 1, dst + 2 * i0, ya);
-                    rope_store8(P.v_pages, 1, dst + 2 * i0 + 8, yz);
+        } else {
+            constexpr int GROUP = D ? D / 16 : 1;
+            uint2 kc[2], vc[2];
+            const int kb = place_codes<GROUP>(xa, xz, kc), vb = place_codes<GROUP>(ya, yz, vc);
+            if (here) {
+                uint8_t* kp = static_cast<uint8_t*>(P.k_pages) + dst;
+                if (ROT == 1) {
+                    *reinterpret_cast<uint2*>(kp + offa) = kc[0];
+                    *reinterpret_cast<uint2*>(kp + offz) = kc[1];
+                } else {
+                    *reinterpret_cast<uint4*>(kp + 2 * i0) = make_uint4(kc[0].x, kc[0].y, kc[1].x, kc[1].y);
                 }
-            } else {
-                constexpr int GROUP = D ? D / 16 : 1;
-                uint2 kc[2], vc[2];
-                const int kb = place_codes<GROUP>(xa, xz, kc), vb = place_codes<GROUP>(ya, yz, vc);
-                if (h0 + u < h_end) {
-                    uint8_t* kp = static_cast<uint8_t*>(P.k_pages) + dst;
-                    if (ROT == 1) {
-                        *reinterpret_cast<uint2*>(kp + offa) = kc[0];
-                        *reinterpret_cast<uint2*>(kp + offz) = kc[1];
-                    } else {
-                        *reinterpret_cast<uint4*>(kp + 2 * i0) = make_uint4(kc[0].x, kc[0].y, kc[1].x, kc[1].y);
-                    }
-                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(P.v_pages) + dst + 2 * i0) = make_uint4(vc[0].x, vc[0].y, vc[1].x, vc[1].y);
-                    if (ch == 0) {
-                        uint8_t* scale = P.scales + tile * 2 * DEC_PT + at % DEC_PT;
-                        scale[0] = (uint8_t)kb;
-                        scale[DEC_PT] = (uint8_t)vb;
-                    }
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(P.v_pages) + dst + 2 * i0) = make_uint4(vc[0].x, vc[0].y, vc[1].x, vc[1].y);
+                if (ch == 0) {
+                    uint8_t* scale = P.scales + tile * 2 * DEC_PT + at % DEC_PT;
+                    scale[0] = (uint8_t)kb;
+                    scale[DEC_PT] = (uint8_t)vb;
                 }
             }
         }
@@ -260,7 +269,7 @@ __global__ void __launch_bounds__(256) place_vec_kernel(const __grid_constant__ 
 __global__ void __launch_bounds__(256) place_rows_kernel(const __grid_constant__ PlaceParams P) {
     if (P.pages) P.lens.publish();
     const int lane = threadIdx.x & 31, half = P.D >> 1;
-    const int heads = P.Hq + (P.pages ? 2 * P.Hkv : 0);
+    const int heads = P.Hq + (P.pages ? 2 : 1) * P.Hkv;
     const long long rows = (long long)P.B * heads * P.n;
     for (long long r = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5; r < rows; r += ((long long)gridDim.x * blockDim.x) >> 5) {
         const int t = (int)(r % P.n);
@@ -283,9 +292,10 @@ __global__ void __launch_bounds__(256) place_rows_kernel(const __grid_constant__
             rope_pair(first ? a : z, first ? z : a, c, s, P.interleaved, ya, yb);
             return first ? ya : yb;
         };
-        if (is_q) {
-            const long long dst = b * P.qos[0] + hk * P.qos[1] + t * P.qos[2];
-            for (int d = lane; d < P.D; d += 32) st_from_float(P.q_out, P.qo_dtype, dst + d, value(d));
+        if (is_q || !P.pages) {
+            const long long* os = is_q ? P.qos : P.vs;
+            const long long dst = b * os[0] + hk * os[1] + t * os[2];
+            for (int d = lane; d < P.D; d += 32) st_from_float(is_q ? P.q_out : P.k_pages, is_q ? P.qo_dtype : P.v_dtype, dst + d, value(d));
             continue;
         }
         const int at = P.lens.before(b) + t;
@@ -304,67 +314,92 @@ __global__ void __launch_bounds__(256) place_rows_kernel(const __grid_constant__
     }
 }
 
-// Dense export of 8-bit pages, as kvcache_gather_kernel: out [B][Hkv][len][D] (strided), rows past a sequence's length are zero.
-struct Gather8Params {
+// Dense export of pages: out [B][Hkv][len][D] (strided), rows past a sequence's length are zero.  The first `front[b]` rows of a
+// sequence's first page have been evicted and are not exported.
+struct GatherPageParams {
     void* k_out;
     void* v_out;
     int k_dtype, v_dtype;
     long long ks[3], vs[3];
-    const int8_t* k_codes;
-    const int8_t* v_codes;
+    const void* k_pages;  // bf16, or codes
+    const void* v_pages;
     const uint8_t* scales;
     const int* page_table;
     const int* end;    // [B]
     const int* front;  // [B]
-    int max_pages, Hkv, D, len, B;
+    int max_pages, Hkv, len, B;
 };
 
-// Four codes times a step: the byte with its sign bit flipped under the exponent of 2^23, which is then taken off.  Exact.
-__device__ __forceinline__ void row8_values(uint32_t codes, float step, float (&f)[4]) {
+// Four codes times a step: the byte with its sign bit flipped under the exponent of 2^23, which is then taken off.  Exact.  BIG: for any
+// step; else for steps up to 2^100, where taking off and multiplying are one operation.
+template <bool BIG>
+__device__ __forceinline__ void row8_values(uint32_t codes, float step, float* f) {
     const uint32_t w = codes ^ 0x80808080u;
+    const float off = -8388736.0f * step;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)) - 8388736.0f) * step;
+    for (int j = 0; j < 4; ++j) {
+        const float x = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j));
+        f[j] = BIG ? (x - 8388736.0f) * step : fmaf(x, step, off);
+    }
 }
 
-// A thread takes 16 codes of a row of K and of V.  vec: rows of the results start on multiples of 16 bytes.  blockIdx.y: (sequence, kv head).
-__global__ void __launch_bounds__(256) kvcache8_gather_kernel(const __grid_constant__ Gather8Params P, const int vec) {
-    const int chunks = P.D / 16;
+// A warp takes a page of K, then of V, all its loads at once, eight elements (16-bit pages) or sixteen (8-bit) per lane.  T: type of the
+// results, whose rows start on multiples of 16 bytes, or 3: any types, any rows.  blockIdx.y: (sequence, kv head).
+template <int PAGES, int D, int T>
+__global__ void __launch_bounds__(256) kvcache_gather_page_kernel(const __grid_constant__ GatherPageParams P) {
+    constexpr int E = PAGES == 2 ? 16 : 8, CH = D / E, ROWS = 32 / CH, N = DEC_PT / ROWS;  // elements of a lane, lanes of a row, rows at once, rounds
+    const int lane = threadIdx.x & 31, c = lane % CH * E, row = lane / CH;
     for (int pair = blockIdx.y; pair < P.B * P.Hkv; pair += gridDim.y) {
         const int b = pair / P.Hkv, hk = pair % P.Hkv, front = __ldg(P.front + b), end = __ldg(P.end + b);
-        for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < (long long)P.len * chunks; i += (long long)gridDim.x * blockDim.x) {
-            const int c = (int)(i % chunks) * 16, t = (int)(i / chunks), at = front + t;
-            uint4 code[2] = {};
-            float step[2] = {0.0f, 0.0f};
-            if (at < end) {
-                const long long tile = (long long)P.page_table[(long long)b * P.max_pages + at / DEC_PT] * P.Hkv + hk;
-                const long long src = (tile * DEC_PT + at % DEC_PT) * P.D + c;
-                code[0] = __ldg(reinterpret_cast<const uint4*>(P.k_codes + src));
-                code[1] = __ldg(reinterpret_cast<const uint4*>(P.v_codes + src));
-                const uint8_t* scale = P.scales + tile * 2 * DEC_PT + at % DEC_PT;
-                step[0] = row8_step(__ldg(scale));
-                step[1] = row8_step(__ldg(scale + DEC_PT));
+        const int pages = (front + P.len + DEC_PT - 1) / DEC_PT;
+        for (int p = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5); p < pages; p += (int)((gridDim.x * blockDim.x) >> 5)) {
+            const bool any = p * DEC_PT < end;
+            const long long tile = any ? (long long)__ldg(P.page_table + (long long)b * P.max_pages + p) * P.Hkv + hk : 0;
+            const float step = any && PAGES == 2 ? row8_step(__ldg(P.scales + tile * 2 * DEC_PT + lane)) : 0.0f;
+            uint4 raw[2][N] = {};
+            if (any) {
+#pragma unroll
+                for (int which = 0; which < 2; ++which)
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        raw[which][j] = __ldcs(reinterpret_cast<const uint4*>(which ? P.v_pages : P.k_pages) + tile * (DEC_PT * D / E) + j * 32 + lane);
             }
+            const auto rows = [&](auto big) {
 #pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                void* out = which ? P.v_out : P.k_out;
-                const int dtype = which ? P.v_dtype : P.k_dtype;
-                const long long* st = which ? P.vs : P.ks;
-                const long long dst = b * st[0] + hk * st[1] + t * st[2] + c;
-                const uint32_t w[4] = {code[which].x, code[which].y, code[which].z, code[which].w};
+                for (int which = 0; which < 2; ++which) {
+                    const long long* st = which ? P.vs : P.ks;
+                    const int dtype = T < 3 ? T : which ? P.v_dtype : P.k_dtype;
+                    void* out = which ? P.v_out : P.k_out;
+                    const long long first = b * st[0] + hk * st[1] + (p * DEC_PT - front) * st[2] + c;
 #pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    float lo[4], hi[4];
-                    row8_values(w[j], step[which], lo);
-                    row8_values(w[j + 1], step[which], hi);
-                    const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                    if (vec) {
-                        rope_store8(out, dtype, dst + 4 * j, f);
-                    } else {
+                    for (int j = 0; j < N; ++j) {
+                        const int at = row + j * ROWS, t = p * DEC_PT + at - front;
+                        const float mine = PAGES == 2 ? __shfl_sync(0xffffffffu, step, which * DEC_PT + at) : 0.0f;
+                        if (t < 0 || t >= P.len) continue;
+                        const uint4 x = p * DEC_PT + at < end ? raw[which][j] : make_uint4(0, 0, 0, 0);  // (codes of 0)
+                        const long long dst = first + at * st[2];
+                        float f[E];
+                        if (PAGES == 2) {
+                            const float by = p * DEC_PT + at < end ? mine : 0.0f;
+                            row8_values<decltype(big)::value>(x.x, by, f);
+                            row8_values<decltype(big)::value>(x.y, by, f + 4);
+                            row8_values<decltype(big)::value>(x.z, by, f + E - 8);
+                            row8_values<decltype(big)::value>(x.w, by, f + E - 4);
+                        } else {
+                            rope_unpack16<false>(x, *reinterpret_cast<float(*)[8]>(f));
+                        }
+                        if (T < 3) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) st_from_float(out, dtype, dst + 4 * j + e, f[e]);
+                            for (int k = 0; k < E; k += 8) rope_store8(out, T, dst + k, *reinterpret_cast<float(*)[8]>(f + k));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) st_from_float(out, dtype, dst + e, f[e]);
+                        }
                     }
                 }
-            }
+            };
+            if (PAGES == 2 && __any_sync(0xffffffffu, !(step <= 0x1p100f))) rows(std::true_type{});
+            else rows(std::false_type{});
         }
     }
 }

@@ -910,44 +910,6 @@ __global__ void kvcache_append_kernel(const __grid_constant__ AppendParams P) {
     }
 }
 
-// Dense export: out [B][Hkv][len][D] (strided, f32 or bf16); rows past a sequence's length are zero.
-// The first `front[b]` rows of a sequence's first page have been evicted and are not exported.
-struct GatherParams {
-    void* k_out;
-    void* v_out;
-    int k_dtype, v_dtype;
-    long long ks[3], vs[3];
-    const __nv_bfloat16* k_pages;
-    const __nv_bfloat16* v_pages;
-    const int* page_table;
-    const int* end;    // [B]
-    const int* front;  // [B]
-    int max_pages, Hkv, D, len, B;
-};
-
-__global__ void kvcache_gather_kernel(const GatherParams P) {
-    const long long total = (long long)P.B * P.Hkv * P.len * P.D;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
-         i += (long long)gridDim.x * blockDim.x) {
-        const int d = (int)(i % P.D);
-        const int t = (int)((i / P.D) % P.len);
-        const int hk = (int)((i / ((long long)P.D * P.len)) % P.Hkv);
-        const int b = (int)(i / ((long long)P.D * P.len * P.Hkv));
-        float kf = 0.0f, vf = 0.0f;
-        const int pos = P.front[b] + t;
-        if (pos < P.end[b]) {
-            const int page = P.page_table[(long long)b * P.max_pages + pos / DEC_PT];
-            const long long src = (((long long)page * P.Hkv + hk) * DEC_PT + pos % DEC_PT) * P.D + d;
-            kf = __bfloat162float(P.k_pages[src]);
-            vf = __bfloat162float(P.v_pages[src]);
-        }
-        const long long kd = b * P.ks[0] + hk * P.ks[1] + t * P.ks[2] + d;
-        const long long vd = b * P.vs[0] + hk * P.vs[1] + t * P.vs[2] + d;
-        st_from_float(P.k_out, P.k_dtype, kd, kf);
-        st_from_float(P.v_out, P.v_dtype, vd, vf);
-    }
-}
-
 // Token-granular eviction of one sequence: rows [drop, drop + keep) of its pages -> dense staging [Hkv][keep][D]
 // (to_pages = 0), then staging -> rows [0, keep) of the same pages (to_pages = 1).  16 bytes per thread and step.
 struct ShiftParams {

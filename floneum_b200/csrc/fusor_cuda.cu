@@ -1341,8 +1341,8 @@ static int32_t kv_reserve(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new
 static bool rope_vec_ok(const void* p, int dtype, const long long* stride);
 
 template <int PAGES, int ROT, int D>
-static void place_vec_run(fusor_cuda_ctx* ctx, const PlaceParams& P, int type, unsigned blocks, unsigned q_blocks, unsigned per) {
-    const auto run = [&](auto kernel) { kernel<<<blocks, 256, 0, ctx->stream>>>(P, q_blocks, per); };
+static void place_vec_run(fusor_cuda_ctx* ctx, const PlaceParams& P, int type, dim3 grid, unsigned q_groups, unsigned per) {
+    const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, ctx->stream>>>(P, q_groups, per); };
     if (type == FUSOR_CUDA_F32) run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_F32, D>);
     else if (type == FUSOR_CUDA_BF16) run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_BF16, D>);
     else run(place_vec_kernel<PAGES, ROT, FUSOR_CUDA_F16, D>);
@@ -1353,17 +1353,17 @@ static int32_t place_launch(fusor_cuda_ctx* ctx, const PlaceParams& P) {
     const int type = P.Hq ? P.q_dtype : P.k_dtype;
     bool vec = P.D % 16 == 0 && reinterpret_cast<uintptr_t>(P.cos_t) % 16 == 0 && reinterpret_cast<uintptr_t>(P.sin_t) % 16 == 0;
     if (P.Hq) vec = vec && P.qo_dtype == type && rope_vec_ok(P.q, type, P.qs) && rope_vec_ok(P.q_out, type, P.qos);
-    if (P.pages) vec = vec && P.k_dtype == type && P.v_dtype == type && rope_vec_ok(P.k_new, type, P.ks) && rope_vec_ok(P.v_new, type, P.vs);
+    if (P.Hkv) vec = vec && P.k_dtype == type && P.v_dtype == type && rope_vec_ok(P.k_new, type, P.ks) && rope_vec_ok(P.pages ? P.v_new : P.k_pages, type, P.vs);
     if (vec) {
-        // eight query heads (half as many kv heads) a thread, halved while fewer than 1024 threads per SM would be left, down to two
-        const long long items = (long long)P.B * P.n * (P.D / 16);
-        const auto q_threads = [&](int per) { return items * ((P.Hq + per - 1) / per); };
-        const auto kv_threads = [&](int per) { return P.pages ? items * ((P.Hkv + per / 2 - 1) / (per / 2)) : 0; };
+        // eight query heads (half as many kv heads that go to pages) a thread, halved while fewer than 512 threads per SM would be left, down to two
+        const long long items = (long long)P.n * (P.D / 16);
+        const auto q_groups = [&](int per) { return (P.Hq + per - 1) / per; };
+        const auto groups = [&](int per) { return q_groups(per) + (P.pages ? (P.Hkv + per / 2 - 1) / (per / 2) : (P.Hkv + per - 1) / per); };
         int per = 8;
-        while (per > 2 && q_threads(per) + kv_threads(per) < 1024ll * ctx->num_sms) per /= 2;
-        const long long q_blocks = (q_threads(per) + 255) / 256, blocks = q_blocks + (kv_threads(per) + 255) / 256;
-        if (blocks <= 0x7fffffffLL) {
-            const auto go = [&](auto run) { run(ctx, P, type, (unsigned)blocks, (unsigned)q_blocks, (unsigned)per); };
+        while (per > 2 && P.B * items * groups(per) < 512ll * ctx->num_sms) per /= 2;
+        if (items < (1ll << 31) && (long long)P.B * groups(per) <= 65535) {
+            const dim3 grid((unsigned)((items + 255) / 256), (unsigned)(P.B * groups(per)));
+            const auto go = [&](auto run) { run(ctx, P, type, grid, (unsigned)q_groups(per), (unsigned)per); };
             if (P.pages == 0) go(P.interleaved ? place_vec_run<0, 2, 0> : place_vec_run<0, 1, 0>);
             else if (P.pages == 1) go(P.interleaved ? place_vec_run<1, 2, 0> : place_vec_run<1, 1, 0>);
             else if (P.D == 128) go(!P.cos_t ? place_vec_run<2, 0, 128> : P.interleaved ? place_vec_run<2, 2, 128> : place_vec_run<2, 1, 128>);
@@ -1371,7 +1371,7 @@ static int32_t place_launch(fusor_cuda_ctx* ctx, const PlaceParams& P) {
             return launch_check(ctx, "place_vec_kernel");
         }
     }
-    const long long rows = (long long)P.B * P.n * (P.Hq + (P.pages ? 2 * P.Hkv : 0));
+    const long long rows = (long long)P.B * P.n * (P.Hq + (P.pages ? 2 : 1) * P.Hkv);
     const int blocks = (int)std::max<long long>(1, std::min<long long>((rows + 7) / 8, (long long)ctx->num_sms * 16));
     place_rows_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
     return launch_check(ctx, "place_rows_kernel");
@@ -1514,6 +1514,24 @@ extern "C" int32_t fusor_cuda_rope_axes(fusor_cuda_ctx* ctx, const fusor_cuda_te
     place_q(P, x, out, cos_t, sin_t, context_length, interleaved);
     P.B = (int)x->shape[0]; P.n = (int)x->shape[2]; P.D = (int)x->shape[3];
     TRY(place_positions(ctx, P, positions, x->shape[3]));
+    return place_launch(ctx, P);
+}
+
+extern "C" int32_t fusor_cuda_rope_axes_qk(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* k, const float* cos_t,
+                                           const float* sin_t, int32_t context_length, const fusor_cuda_rope_positions* positions,
+                                           int32_t interleaved, const fusor_cuda_tensor4* q_out, const fusor_cuda_tensor4* k_out) {
+    if (!ctx) return fail(nullptr, FUSOR_CUDA_INVALID_ARGUMENT, "ctx is null");
+    TRY(rope_check(ctx, q, q_out, cos_t, sin_t, context_length, "q"));
+    TRY(rope_check(ctx, k, k_out, cos_t, sin_t, context_length, "k"));
+    if (k->shape[0] != q->shape[0] || k->shape[2] != q->shape[2] || k->shape[3] != q->shape[3])
+        return fail(ctx, FUSOR_CUDA_SHAPE_MISMATCH, "q and k differ in batch, tokens or head_dim");
+    DeviceGuard g(ctx->device);
+    PlaceParams P{};
+    place_q(P, q, q_out, cos_t, sin_t, context_length, interleaved);
+    P.B = (int)q->shape[0]; P.n = (int)q->shape[2]; P.D = (int)q->shape[3];
+    P.k_new = k->data; P.k_pages = k_out->data; P.k_dtype = k->dtype; P.v_dtype = k_out->dtype; P.Hkv = (int)k->shape[1];
+    for (int i = 0; i < 3; ++i) { P.ks[i] = k->stride[i]; P.vs[i] = k_out->stride[i]; }
+    TRY(place_positions(ctx, P, positions, q->shape[3]));
     return place_launch(ctx, P);
 }
 
@@ -1714,27 +1732,26 @@ extern "C" int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* c, const fusor_
     if (k_out->stride[3] != 1 || v_out->stride[3] != 1) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "the head_dim axis must be contiguous");
     DeviceGuard g(ctx->device);
     TRY(kv_sync_tables(c));
-    const long long total = (long long)c->active_B * c->Hkv * longest * c->D;
-    if (c->k_codes) {
-        Gather8Params P;
-        P.k_out = k_out->data; P.v_out = v_out->data; P.k_dtype = k_out->dtype; P.v_dtype = v_out->dtype;
-        for (int i = 0; i < 3; ++i) { P.ks[i] = k_out->stride[i]; P.vs[i] = v_out->stride[i]; }
-        P.k_codes = c->k_codes; P.v_codes = c->v_codes; P.scales = c->scales; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
-        P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.D = c->D; P.len = longest; P.B = c->active_B;
-        if (total == 0) return FUSOR_CUDA_OK;
-        const bool vec = rope_vec_ok(P.k_out, P.k_dtype, P.ks) && rope_vec_ok(P.v_out, P.v_dtype, P.vs);
-        const long long threads = (long long)longest * (c->D / 16);
-        const dim3 grid((unsigned)std::min<long long>((threads + 255) / 256, 1 << 20), (unsigned)std::min(P.B * P.Hkv, 65535));
-        kvcache8_gather_kernel<<<grid, (unsigned)std::min<long long>(256, (threads + 31) / 32 * 32), 0, ctx->stream>>>(P, vec ? 1 : 0);
-        return launch_check(ctx, "kvcache8_gather_kernel");
-    }
-    GatherParams P;
+    if (longest == 0) return FUSOR_CUDA_OK;
+    GatherPageParams P;
     P.k_out = k_out->data; P.v_out = v_out->data; P.k_dtype = k_out->dtype; P.v_dtype = v_out->dtype;
     for (int i = 0; i < 3; ++i) { P.ks[i] = k_out->stride[i]; P.vs[i] = v_out->stride[i]; }
-    P.k_pages = c->k_pages; P.v_pages = c->v_pages; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
-    P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.D = c->D; P.len = longest; P.B = c->active_B;
-    const int blocks = (int)std::min<long long>((total + 255) / 256, (long long)ctx->num_sms * 8);
-    kvcache_gather_kernel<<<blocks, 256, 0, ctx->stream>>>(P);
+    P.k_pages = kv_pool(c, 0); P.v_pages = kv_pool(c, 1); P.scales = c->scales; P.page_table = c->d_page_table; P.end = c->d_end; P.front = c->d_front;
+    P.max_pages = c->max_pages; P.Hkv = c->Hkv; P.len = longest; P.B = c->active_B;
+    const bool vec = P.k_dtype == P.v_dtype && rope_vec_ok(P.k_out, P.k_dtype, P.ks) && rope_vec_ok(P.v_out, P.v_dtype, P.vs);
+    const unsigned warps = (unsigned)pages_of(longest + DEC_PT - 1);  // a page each (evicted rows may begin the first)
+    const dim3 grid((warps + 7) / 8, (unsigned)std::min(P.B * P.Hkv, 65535));
+    const auto run = [&](auto f32, auto bf16, auto f16, auto any) {
+        (!vec ? any : P.k_dtype == FUSOR_CUDA_F32 ? f32 : P.k_dtype == FUSOR_CUDA_BF16 ? bf16 : f16)<<<grid, std::min(warps, 8u) * 32, 0, ctx->stream>>>(P);
+    };
+    if (c->k_codes && c->D == 128)
+        run(kvcache_gather_page_kernel<2, 128, 0>, kvcache_gather_page_kernel<2, 128, 1>, kvcache_gather_page_kernel<2, 128, 2>, kvcache_gather_page_kernel<2, 128, 3>);
+    else if (c->k_codes)
+        run(kvcache_gather_page_kernel<2, 64, 0>, kvcache_gather_page_kernel<2, 64, 1>, kvcache_gather_page_kernel<2, 64, 2>, kvcache_gather_page_kernel<2, 64, 3>);
+    else if (c->D == 128)
+        run(kvcache_gather_page_kernel<1, 128, 0>, kvcache_gather_page_kernel<1, 128, 1>, kvcache_gather_page_kernel<1, 128, 2>, kvcache_gather_page_kernel<1, 128, 3>);
+    else
+        run(kvcache_gather_page_kernel<1, 64, 0>, kvcache_gather_page_kernel<1, 64, 1>, kvcache_gather_page_kernel<1, 64, 2>, kvcache_gather_page_kernel<1, 64, 3>);
     return launch_check(ctx, "kvcache_gather_kernel");
 }
 

@@ -68,8 +68,7 @@ def axes_of_sections(sections: Sequence[int], alternating: bool = False) -> np.n
 
 
 def _positions(positions: Tensor, axes, batch: int, n: int, head_dim: int):
-    """The C view of positions (u32 [n_axes, n], the same for every sequence, or [n_axes, batch, n]); keep the second value
-    alive until the call has returned."""
+    """The C view of positions (u32 [n_axes, n], the same for every sequence, or [n_axes, batch, n])."""
     assert positions.dtype == U32, "positions must be a u32 tensor"
     shape, strides = positions.shape(), positions.strides
     assert len(shape) in (2, 3) and shape[-1] == n and (len(shape) == 2 or shape[1] == batch), (
@@ -79,8 +78,8 @@ def _positions(positions: Tensor, axes, batch: int, n: int, head_dim: int):
     assert axis_of_pair.shape == (head_dim // 2,), f"axes must name the axis of each of {head_dim // 2} pairs, got {list(axis_of_pair.shape)}"
     p = _lib.RopePositions()
     p.ids, p.axis_stride, p.batch_stride = positions.ptr, strides[0], strides[1] if len(shape) == 3 else 0
-    p.n_axes, p.axis_of_pair = shape[0], axis_of_pair.ctypes.data
-    return p, axis_of_pair
+    p.n_axes, p.axis_of_pair = shape[0], axis_of_pair.tobytes()  # (the structure keeps the bytes)
+    return p
 
 
 def rope_axes(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, axes, interleaved: bool = False,
@@ -93,7 +92,7 @@ def rope_axes(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, axes, inte
     assert len(shape) == 4, "rope expects [batch, heads, sequence, head_dim]"
     assert shape[3] % 2 == 0, "head_dim must be even"
     _check_tables(cos, sin, shape[3])
-    pos, keep = _positions(positions, axes, shape[0], shape[2], shape[3])
+    pos = _positions(positions, axes, shape[0], shape[2], shape[3])
     dev = x.device
     out = Tensor.empty(dev, shape, x.dtype if out_dtype is None else out_dtype)
     cx, co = x._c4(), out._c4()
@@ -128,9 +127,20 @@ class RopeCache:
         return (rope(q, self.cos, self.sin, start_pos, True), rope(k, self.cos, self.sin, start_pos, True))
 
     def forward_axes(self, q: Tensor, k: Tensor, positions: Tensor, axes, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
-        """`forward` for tokens with a position on each of several axes (time, row, column): see `rope_axes`."""
-        return (rope_axes(q, self.cos, self.sin, positions, axes, interleaved),
-                rope_axes(k, self.cos, self.sin, positions, axes, interleaved))
+        """`forward` for tokens with a position on each of several axes (time, row, column), in one launch: see `rope_axes`."""
+        B, _, n, D = q.shape()
+        kB, _, kn, kD = k.shape()
+        assert (kB, kn, kD) == (B, n, D), f"q {list(q.shape())} and k {list(k.shape())} differ in batch, tokens or head_dim"
+        assert D % 2 == 0, "head_dim must be even"
+        _check_tables(self.cos, self.sin, D)
+        pos = _positions(positions, axes, B, n, D)
+        dev = q.device
+        q_out, k_out = Tensor.empty(dev, q.shape(), q.dtype), Tensor.empty(dev, k.shape(), k.dtype)
+        cq, ck, cqo, cko = q._c4(), k._c4(), q_out._c4(), k_out._c4()
+        _lib.check(_lib.load().fusor_cuda_rope_axes_qk(dev.handle, ctypes.byref(cq), ctypes.byref(ck), self.cos.ptr, self.sin.ptr,
+                                                       self.cos.shape()[0], ctypes.byref(pos), int(bool(interleaved)),
+                                                       ctypes.byref(cqo), ctypes.byref(cko)), dev.handle)
+        return q_out, k_out
 
     def forward_append(self, q: Tensor, k: Tensor, v: Tensor, cache, start_pos: int = -1, interleaved: bool = False,
                        out_dtype: int | None = None, positions: Optional[Tensor] = None, axes=None):

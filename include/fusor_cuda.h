@@ -237,6 +237,10 @@ typedef struct fusor_cuda_rope_positions {
 /* fusor_cuda_rope with such positions in place of start_pos + t; head_dim up to 512. */
 int32_t fusor_cuda_rope_axes(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* x, const float* cos, const float* sin, int32_t context_length,
                              const fusor_cuda_rope_positions* positions, int32_t interleaved, const fusor_cuda_tensor4* out);
+/* The same for q and k of one layer (batch, tokens and head_dim agree), in one launch. */
+int32_t fusor_cuda_rope_axes_qk(fusor_cuda_ctx* ctx, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* k, const float* cos,
+                                const float* sin, int32_t context_length, const fusor_cuda_rope_positions* positions, int32_t interleaved,
+                                const fusor_cuda_tensor4* q_out, const fusor_cuda_tensor4* k_out);
 /* fusor_cuda_kvcache_rope_append with such positions: q -> q_out, rotated k and v -> the cache, either kind, in one launch. */
 int32_t fusor_cuda_kvcache_rope_axes_append(fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* q, const fusor_cuda_tensor4* k_new,
                                             const fusor_cuda_tensor4* v_new, const float* cos, const float* sin, int32_t context_length,

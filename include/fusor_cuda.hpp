@@ -469,18 +469,22 @@ struct RopeAxes {
     bool per_sequence = false;  // ids has the batch axis
     int32_t n_axes = 0;
     std::vector<uint8_t> axis_of_pair;
+    fusor_cuda_rope_positions view(const std::array<int64_t, 4>& shape) const {
+        if ((int64_t)axis_of_pair.size() * 2 != shape[3]) throw std::logic_error("rope_axes: axis_of_pair must name the axis of each pair");
+        fusor_cuda_rope_positions pos{};
+        pos.ids = ids;
+        pos.axis_stride = shape[2] * (per_sequence ? shape[0] : 1);
+        pos.batch_stride = per_sequence ? shape[2] : 0;
+        pos.n_axes = n_axes;
+        pos.axis_of_pair = axis_of_pair.data();
+        return pos;
+    }
 };
 inline Tensor<4> rope_axes(const Tensor<4>& x, const Tensor<2>& cos, const Tensor<2>& sin, const RopeAxes& axes, bool interleaved = false) {
     if (cos.shape() != sin.shape() || cos.shape()[1] * 2 != x.shape()[3]) throw std::logic_error("rope: cos / sin must be [context, head_dim / 2]");
-    if ((int64_t)axes.axis_of_pair.size() * 2 != x.shape()[3]) throw std::logic_error("rope_axes: axis_of_pair must name the axis of each pair");
     Tensor<4> out = Tensor<4>::empty(x.device(), x.shape(), x.dtype());
     const fusor_cuda_tensor4 vx = detail::view4(x), vo = detail::view4(out);
-    fusor_cuda_rope_positions pos{};
-    pos.ids = axes.ids;
-    pos.axis_stride = x.shape()[2] * (axes.per_sequence ? x.shape()[0] : 1);
-    pos.batch_stride = axes.per_sequence ? x.shape()[2] : 0;
-    pos.n_axes = axes.n_axes;
-    pos.axis_of_pair = axes.axis_of_pair.data();
+    const fusor_cuda_rope_positions pos = axes.view(x.shape());
     x.device()->check(fusor_cuda_rope_axes(x.device()->raw(), &vx, static_cast<const float*>(cos.data()), static_cast<const float*>(sin.data()),
                                            (int32_t)cos.shape()[0], &pos, interleaved ? 1 : 0, &vo));
     return out;
@@ -509,7 +513,16 @@ class RopeCache {
         return {rope(q, cos_, sin_, start_pos, true), rope(k, cos_, sin_, start_pos, true)};
     }
     std::pair<Tensor<4>, Tensor<4>> forward_axes(const Tensor<4>& q, const Tensor<4>& k, const RopeAxes& axes, bool interleaved = false) const {
-        return {rope_axes(q, cos_, sin_, axes, interleaved), rope_axes(k, cos_, sin_, axes, interleaved)};
+        const auto &qs = q.shape(), &ks = k.shape();
+        if (ks[0] != qs[0] || ks[2] != qs[2] || ks[3] != qs[3]) throw std::logic_error("forward_axes: q and k differ in batch, tokens or head_dim");
+        if (cos_.shape() != sin_.shape() || cos_.shape()[1] * 2 != qs[3]) throw std::logic_error("rope: cos / sin must be [context, head_dim / 2]");
+        const fusor_cuda_rope_positions pos = axes.view(q.shape());
+        Tensor<4> q_out = Tensor<4>::empty(q.device(), qs, q.dtype()), k_out = Tensor<4>::empty(q.device(), ks, k.dtype());
+        const fusor_cuda_tensor4 vq = detail::view4(q), vk = detail::view4(k), vqo = detail::view4(q_out), vko = detail::view4(k_out);
+        q.device()->check(fusor_cuda_rope_axes_qk(q.device()->raw(), &vq, &vk, static_cast<const float*>(cos_.data()),
+                                                  static_cast<const float*>(sin_.data()), (int32_t)cos_.shape()[0], &pos, interleaved ? 1 : 0,
+                                                  &vqo, &vko));
+        return {q_out, k_out};
     }
     const Tensor<2>& cos() const { return cos_; }
     const Tensor<2>& sin() const { return sin_; }

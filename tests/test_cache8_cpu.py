@@ -29,11 +29,11 @@ def test_positions_are_checked_before_the_call():
     from floneum_b200.rope import _positions
     ids = lambda *shape, **kw: fb.Tensor(None, 4096, shape, kw.pop("dtype", fb.U32), **kw)
     axes = fb.axes_of_sections([2, 2])
-    p, keep = _positions(ids(2, 3, 5), axes, 3, 5, 8)
+    p = _positions(ids(2, 3, 5), axes, 3, 5, 8)
     assert (p.ids, p.axis_stride, p.batch_stride, p.n_axes) == (4096, 15, 5, 2)
-    p, keep = _positions(ids(2, 5), axes, 3, 5, 8)
+    p = _positions(ids(2, 5), axes, 3, 5, 8)
     assert (p.axis_stride, p.batch_stride) == (5, 0)
-    p, keep = _positions(ids(2, 3, 5, strides=(40, 8, 1)), axes, 3, 5, 8)
+    p = _positions(ids(2, 3, 5, strides=(40, 8, 1)), axes, 3, 5, 8)
     assert (p.axis_stride, p.batch_stride) == (40, 8)
     for bad in (ids(2, 3, 5, dtype=fb.F32), ids(2, 3, 4), ids(2, 2, 5), ids(5), ids(2, 3, 5, strides=(30, 10, 2))):
         with pytest.raises(AssertionError):

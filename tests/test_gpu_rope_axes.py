@@ -68,6 +68,24 @@ def test_one_position_on_every_axis_is_rope(device):
         assert all(np.array_equal(x.as_slice(), y.as_slice()) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,n,D,sections", [(1, 16, 16, 70, 80, [20, 20]), (2, 14, 2, 33, 128, [16, 24, 24]), (3, 3, 1, 1, 64, [32]), (2, 4, 2, 9, 6, [1, 2]),
+                                                   (1, 1, 9, 300, 96, [24, 24])])
+def test_q_and_k_in_one_call(device, B, Hq, Hkv, n, D, sections):
+    fb = _fb()
+    rng = np.random.default_rng(D * n)
+    cos, sin = (rng.uniform(-1, 1, (90, D // 2)).astype(np.float32) for _ in range(2))
+    rope, axes = fb.RopeCache.from_parts(_T(device, cos), _T(device, sin)), fb.axes_of_sections(sections)
+    ids = rng.integers(0, 90, (len(sections), B, n)).astype(np.uint32)
+    for dtypes in ((0, 0), (1, 1), (2, 2), (0, 1)):
+        q, k = (_as(rng.standard_normal((B, h, n, D)).astype(np.float32), t) for h, t in zip((Hq, Hkv), dtypes))
+        for interleaved in (False, True):
+            got = rope.forward_axes(_T(device, q, dtypes[0]), _T(device, k, dtypes[1]), _T(device, ids, fb.U32), axes, interleaved)
+            for g, x, t in zip(got, (q, k), dtypes):
+                assert np.array_equal(g.as_slice(), _as(_turn(x, cos, sin, ids, axes, interleaved), t))
+    with pytest.raises(AssertionError):
+        rope.forward_axes(_T(device, q), _T(device, np.zeros((B, Hkv, n + 1, D), np.float32)), _T(device, ids, fb.U32), axes)
+
+
 def test_strided_views(device):
     """Heads behind tokens in memory, rows that start one element off, positions cut out of longer ones; nothing else is written."""
     import torch
@@ -87,7 +105,7 @@ def test_strided_views(device):
             co, x4, o4 = [fb.Tensor.from_torch(device, t) for t in (cos, sin)], fb.Tensor.from_torch(device, x), fb.Tensor.from_torch(device, view)
             import ctypes
             from floneum_b200.rope import _positions
-            pos, keep = _positions(fb.Tensor.from_torch(device, ids[:, :, 5:5 + n]), axes, B, n, D)
+            pos = _positions(fb.Tensor.from_torch(device, ids[:, :, 5:5 + n]), axes, B, n, D)
             cx, c_o = x4._c4(), o4._c4()
             L = fb._lib.load()
             fb._lib.check(L.fusor_cuda_rope_axes(device.handle, ctypes.byref(cx), co[0].ptr, co[1].ptr, rows, ctypes.byref(pos), 0, ctypes.byref(c_o)),
@@ -219,7 +237,7 @@ def test_refusals(device):
 
     def rc(**kw):
         p = fb._lib.RopePositions()
-        p.ids, p.axis_stride, p.batch_stride, p.n_axes, p.axis_of_pair = ids.ptr, 4, 0, 2, axes.ctypes.data
+        p.ids, p.axis_stride, p.batch_stride, p.n_axes, p.axis_of_pair = ids.ptr, 4, 0, 2, axes.tobytes()
         for k, v in kw.items():
             setattr(p, k, v)
         cx, co = x._c4(), x._c4()
