@@ -346,7 +346,7 @@ __device__ __forceinline__ void row8_values(uint32_t codes, float step, float* f
 // A warp takes a page of K, then of V, all its loads at once, eight elements (16-bit pages) or sixteen (8-bit) per lane.  T: type of the
 // results, whose rows start on multiples of 16 bytes, or 3: any types, any rows.  blockIdx.y: (sequence, kv head).
 template <int PAGES, int D, int T>
-__global__ void __launch_bounds__(256) kvcache_gather_page_kernel(const __grid_constant__ GatherPageParams P) {
+__global__ void __launch_bounds__(256, 4) kvcache_gather_page_kernel(const __grid_constant__ GatherPageParams P) {
     constexpr int E = PAGES == 2 ? 16 : 8, CH = D / E, ROWS = 32 / CH, N = DEC_PT / ROWS;  // elements of a lane, lanes of a row, rows at once, rounds
     const int lane = threadIdx.x & 31, c = lane % CH * E, row = lane / CH;
     for (int pair = blockIdx.y; pair < P.B * P.Hkv; pair += gridDim.y) {
@@ -356,50 +356,50 @@ __global__ void __launch_bounds__(256) kvcache_gather_page_kernel(const __grid_c
             const bool any = p * DEC_PT < end;
             const long long tile = any ? (long long)__ldg(P.page_table + (long long)b * P.max_pages + p) * P.Hkv + hk : 0;
             const float step = any && PAGES == 2 ? row8_step(__ldg(P.scales + tile * 2 * DEC_PT + lane)) : 0.0f;
-            uint4 raw[2][N] = {};
-            if (any) {
+            const auto rows = [&](int which, auto big) {
+                uint4 raw[N] = {};
+                if (any) {
+                    const uint4* from = reinterpret_cast<const uint4*>(which ? P.v_pages : P.k_pages) + tile * (DEC_PT * D / E) + lane;
 #pragma unroll
-                for (int which = 0; which < 2; ++which)
+                    for (int j = 0; j < N; ++j) raw[j] = __ldcs(from + j * 32);
+                }
+                const long long* st = which ? P.vs : P.ks;
+                const int dtype = T < 3 ? T : which ? P.v_dtype : P.k_dtype;
+                void* out = which ? P.v_out : P.k_out;
+                const long long first = b * st[0] + hk * st[1] + (p * DEC_PT - front) * st[2] + c;
 #pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        raw[which][j] = __ldcs(reinterpret_cast<const uint4*>(which ? P.v_pages : P.k_pages) + tile * (DEC_PT * D / E) + j * 32 + lane);
-            }
-            const auto rows = [&](auto big) {
+                for (int j = 0; j < N; ++j) {
+                    const int at = row + j * ROWS, t = p * DEC_PT + at - front;
+                    const float mine = PAGES == 2 ? __shfl_sync(0xffffffffu, step, which * DEC_PT + at) : 0.0f;
+                    if (t < 0 || t >= P.len) continue;
+                    const bool there = p * DEC_PT + at < end;
+                    const uint4 x = there ? raw[j] : make_uint4(0, 0, 0, 0);  // (codes of 0)
+                    const long long dst = first + at * st[2];
+                    float f[E];
+                    if (PAGES == 2) {
+                        const float by = there ? mine : 0.0f;
+                        row8_values<decltype(big)::value>(x.x, by, f);
+                        row8_values<decltype(big)::value>(x.y, by, f + 4);
+                        row8_values<decltype(big)::value>(x.z, by, f + E - 8);
+                        row8_values<decltype(big)::value>(x.w, by, f + E - 4);
+                    } else {
+                        rope_unpack16<false>(x, *reinterpret_cast<float(*)[8]>(f));
+                    }
+                    if (T < 3) {
 #pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    const long long* st = which ? P.vs : P.ks;
-                    const int dtype = T < 3 ? T : which ? P.v_dtype : P.k_dtype;
-                    void* out = which ? P.v_out : P.k_out;
-                    const long long first = b * st[0] + hk * st[1] + (p * DEC_PT - front) * st[2] + c;
+                        for (int k = 0; k < E; k += 8) rope_store8(out, T, dst + k, *reinterpret_cast<float(*)[8]>(f + k));
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const int at = row + j * ROWS, t = p * DEC_PT + at - front;
-                        const float mine = PAGES == 2 ? __shfl_sync(0xffffffffu, step, which * DEC_PT + at) : 0.0f;
-                        if (t < 0 || t >= P.len) continue;
-                        const uint4 x = p * DEC_PT + at < end ? raw[which][j] : make_uint4(0, 0, 0, 0);  // (codes of 0)
-                        const long long dst = first + at * st[2];
-                        float f[E];
-                        if (PAGES == 2) {
-                            const float by = p * DEC_PT + at < end ? mine : 0.0f;
-                            row8_values<decltype(big)::value>(x.x, by, f);
-                            row8_values<decltype(big)::value>(x.y, by, f + 4);
-                            row8_values<decltype(big)::value>(x.z, by, f + E - 8);
-                            row8_values<decltype(big)::value>(x.w, by, f + E - 4);
-                        } else {
-                            rope_unpack16<false>(x, *reinterpret_cast<float(*)[8]>(f));
-                        }
-                        if (T < 3) {
-#pragma unroll
-                            for (int k = 0; k < E; k += 8) rope_store8(out, T, dst + k, *reinterpret_cast<float(*)[8]>(f + k));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; ++e) st_from_float(out, dtype, dst + e, f[e]);
-                        }
+                        for (int e = 0; e < E; ++e) st_from_float(out, dtype, dst + e, f[e]);
                     }
                 }
             };
-            if (PAGES == 2 && __any_sync(0xffffffffu, !(step <= 0x1p100f))) rows(std::true_type{});
-            else rows(std::false_type{});
+            const bool big = PAGES == 2 && __any_sync(0xffffffffu, !(step <= 0x1p100f));
+#pragma unroll 1
+            for (int which = 0; which < 2; ++which) {
+                if (big) rows(which, std::true_type{});
+                else rows(which, std::false_type{});
+            }
         }
     }
 }
