@@ -565,7 +565,7 @@ struct Decode8Records {
 // of eight records do not wait for their weights.
 template <int D>
 __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const Decode8Records& R, int pair, int rr, int lane) {
-    constexpr int E = D / 32, BATCH = 8;
+        constexpr int E = D / 32, BATCH = 8;
     const int b = pair / P.Hkv, hk = pair % P.Hkv;
     float M = -INFINITY, L = 0.0f, acc[E] = {};
     for (int i0 = 0; i0 < R.n; i0 += BATCH) {
@@ -577,11 +577,12 @@ __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const D
         for (int k = 0; k < BATCH; ++k) {
             const float* from = P.part_o + __shfl_sync(0xffffffffu, row, k) * D + lane * E;  // (past the last record: the last one's)
             if (k < here) {
-#pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(from + e));
-                    o[k][e] = y.x;
-                    o[k][e + 1] = y.y;
+                if (E == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(from));
+                    o[k][0] = y.x; o[k][1] = y.y; o[k][E - 2] = y.z; o[k][E - 1] = y.w;
+                } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
+                    o[k][0] = y.x; o[k][1] = y.y;
                 }
             }
         }

@@ -1927,13 +1927,20 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
     fusor_cuda_ctx* ctx = c->ctx;
     long long longest = 0;
     for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
-    const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;
+    const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;  // bytes of a page pair
+    // CTAs of the even deal: a record per CTA and pair, which one CTA merges, so not more than 32 to a pair (one sequence of 64000
+    // tokens with one kv head: 45 us from 148 CTAs, 27 from 32)
+    const int grid = c->decode_ctas > 0 ? c->decode_ctas : (int)std::min<long long>(ctx->num_sms, 32 * heads);
+    // A cluster per (sequence, kv head), of the largest size of which all fit at once, while its longest share is short enough.  Measured
+    // (ns, 4 KB page pairs): the cluster 7200 + 93 per page of that share, the deal 13000 + 98 per page of a CTA's.  One sequence of
+    // 1411 tokens 7.9 against 12.2 us, of 12000 15.9 and 19.1, of 24000 23.1 and 22.4; four of 8192 19.5 and 22.5; sixteen of 256 .. 4096
+    // 28.1 and 25.1 (32 query heads on 8 of 128, graphs, pages cold).
     if (P.res.mode != 2 && c->decode_ctas == 0 && heads <= ctx->num_sms && longest >= 1) {
         int i = 0;
         while (i < 3 && heads <= ctx->clusters[i + 1]) ++i;
         const int C = 1 << i;
-        const long long share = (longest + C - 1) / C, share_ns = share * std::max<long long>(126, 161 * heads * C / 128) * unit / 8192;
-        if (share_ns <= 9300 + total * 194 / ctx->num_sms * unit / 8192) {
+        const long long share = (longest + C - 1) / C;
+        if (7200 + 93 * share * unit / 4096 <= 13000 + 98 * total / grid * unit / 4096) {
             cudaLaunchAttribute attr;
             const cudaLaunchConfig_t cfg = cluster_config(ctx, (unsigned)(heads * C), (unsigned)C, D8_THREADS,
                                                           c->D == 128 ? Decode8ClusterSmem<128>::bytes : Decode8ClusterSmem<64>::bytes, &attr);
@@ -1941,9 +1948,7 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
             return launch_check(ctx, "decode8_cluster_kernel");
         }
     }
-    // every warp its share, at least a page of it
-    const int grid = c->decode_ctas > 0 ? c->decode_ctas : ctx->num_sms;
-    const int shares = (int)std::min<long long>((long long)grid * D8_NW, total);
+    const int shares = (int)std::min<long long>((long long)grid * D8_NW, total);  // every warp its share, at least a page of it
     if (total > 0) {  // (every chunk empty: only the merge kernel runs and writes empty records)
         const auto run = [&](auto kernel, size_t smem) { kernel<<<(shares + D8_NW - 1) / D8_NW, D8_THREADS, smem, ctx->stream>>>(P, shares); };
         if (c->D == 128) run(decode8_splitkv_kernel<128>, Decode8Smem<128>::bytes);

@@ -40,5 +40,5 @@ def attention_bound(q, k, v, scale):
     query in two 11-bit terms adds 2^-21), which the exponential turns into the same error relative to each weight, for the
     weight and for the sum; exponentials, two-term weights and the sums themselves 2^-19 on top, of the largest |v|."""
     D = q.shape[-1]
-    s = np.einsum("hd,hnd->hn", np.abs(np.asarray(q, np.float64)), np.repeat(np.abs(np.asarray(k, np.float64)), q.shape[0] // k.shape[0], 0)) * scale
+    s = np.einsum("hd,hnd->hn", np.abs(np.asarray(q, np.float64)), np.repeat(np.abs(np.asarray(k, np.float64)), q.shape[0] // k.shape[0], 0)) * abs(scale)
     return (2 * s.max() * ((D + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -19) * np.abs(np.asarray(v, np.float64)).max()

@@ -433,6 +433,110 @@ def test_two_decodes_at_once_and_a_replayed_one(device):
     del graph
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_sequences_than_warps(device, D):
+    """Hundreds of sequences of a token to three pages: shares that hold many of them whole."""
+    rng = np.random.default_rng(300 + D)
+    lens = [int(x) for x in rng.integers(1, 41, 300)]
+    cache, rows = _filled(device, rng, lens, 4, D)
+    q = rng.standard_normal((300, 8, 1, D)).astype(np.float32)
+    for ctas in (0, 3, 148, 0):
+        cache.set_decode_ctas(ctas)
+        _check(cache.decode(_T(device, q), float(D ** -0.5)).as_slice(), q, rows, float(D ** -0.5), 0)
+
+
+def test_one_cache_at_one_grid_after_another(device):
+    """What a launch leaves behind for the next: the same result from every grid, again and again, and as captured."""
+    import torch
+    fb = _fb()
+    stream = torch.cuda.Stream()
+    dev = fb.Device.gpu(0, stream.cuda_stream)
+    rng = np.random.default_rng(41)
+    cache, rows = _filled(dev, rng, [5000, 7, 900, 16, 3100], 3, 128)
+    q = rng.standard_normal((5, 12, 1, 128)).astype(np.float32)
+    tq = _T(dev, q)
+    first = {}
+    for ctas in (148, 1, 40, 148, 9, 0, 40, 1, 9, 0):
+        cache.set_decode_ctas(ctas)
+        got = cache.decode(tq, 0.09).as_slice()
+        _check(got, q, rows, 0.09, 0)
+        assert np.array_equal(got, first.setdefault(ctas, got))
+    for ctas in (40, 0):
+        cache.set_decode_ctas(ctas)
+        out = fb.Tensor.zeros(dev, q.shape)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+            for _ in range(3):
+                cache.decode(tq, 0.09, out=out)
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(out.as_slice(), first[ctas])
+        del graph
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_any_scale_and_a_query_of_zeros(device, scale):
+    rng = np.random.default_rng(2)
+    cache, rows = _filled(device, rng, [300, 5], 2, 64)
+    q = rng.standard_normal((2, 6, 1, 64)).astype(np.float32)
+    q[0, 1] = 0
+    _check(cache.decode(_T(device, q), scale).as_slice(), q, rows, scale, 0)
+
+
+def test_exchange_decode_of_one_rank(device):
+    """The KV-chunk decode's merge and exchange over 8-bit pages, with a sequence of which this rank has no key."""
+    fb = _fb()
+    from floneum_b200.sharding import PeerExchange
+    rng = np.random.default_rng(19)
+    lens = [3000, 20, 700]
+    cache, rows = _filled(device, rng, lens, 2, 128)
+    q = rng.standard_normal((3, 8, 1, 128)).astype(np.float32)
+    ex = PeerExchange(device, 0, 1, 3 * 8 * 130)
+    for ctas in (0, 5, 148, 0):
+        cache.set_decode_ctas(ctas)
+        out = fb.Tensor.zeros(device, (3, 8, 128))
+        ex.decode(cache, _T(device, q), 0.09, out)
+        _check(out.as_slice()[:, :, None], q, rows, 0.09, 0)
+    empty = fb.PagedKvCache(device, 3, 2, 128, 4, 2, dtype=fb.I8)
+    empty.set_page_table(np.array([[0, 1], [0, 0], [2, 0]], np.int32), np.array([20, 0, 3], np.int32))
+    for _ in range(2):
+        out = fb.Tensor.from_slice(device, (3, 8, 128), np.full((3, 8, 128), 7.0))
+        ex.decode(empty, _T(device, q), 0.09, out)
+        assert not out.as_slice().any()  # rows of zeros, and no rows
+    ex.close()
+
+
+def test_pools_of_more_than_four_gigabytes(device):
+    """Pages behind byte 2^32 of a pool: written, rotated into, read back, moved and attended over."""
+    fb = _fb()
+    rng = np.random.default_rng(44)
+    pages, Hkv, D = 270000, 8, 128  # 4.4 GB a pool
+    assert pages * Hkv * 16 * D > 2 ** 32
+    cache = fb.PagedKvCache(device, 1, Hkv, D, pages, 4, dtype=fb.I8)
+    rope = fb.RopeCache.new(D, 64, 10000.0, device)
+    k, v = (rng.standard_normal((1, Hkv, 33, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((1, 8, 12, D)).astype(np.float32)
+    cache.set_page_table(np.array([[pages - 1, 0, 0, 0]], np.int32), np.array([1], np.int32))
+    cache.append(_T(device, k[:, :, :15].copy()), _T(device, v[:, :, :15].copy()))
+    cache.set_page_table(np.array([[pages - 1, 3, pages - 2, 0]], np.int32), np.array([33], np.int32))
+    cache.append(_T(device, k[:, :, 15:18].copy()), _T(device, v[:, :, 15:18].copy()))
+    cache.rope_append(_T(device, q), _T(device, k[:, :, 21:33].copy()), _T(device, v[:, :, 21:33].copy()), rope.cos, rope.sin, 5)
+    gk, gv = (x.as_slice() for x in cache.gather(1, 48))
+    zero = np.zeros_like(k[:, :, :1])
+    want_k = np.concatenate([zero, held(k[:, :, :15]), np.repeat(zero, 17, 2), held(k[:, :, 15:18]),
+                             held(O.rope(k[:, :, 21:33], rope.cos.as_slice(), rope.sin.as_slice(), 5, False))], 2)
+    want_v = np.concatenate([zero, held(v[:, :, :15]), np.repeat(zero, 17, 2), held(v[:, :, 15:18]), held(v[:, :, 21:33])], 2)
+    assert np.array_equal(gk, want_k) and np.array_equal(gv, want_v)
+    one = q[:, :, :1].copy()
+    for ctas in (0, 2):
+        cache.set_decode_ctas(ctas)
+        _check(cache.decode(_T(device, one), 0.09).as_slice(), one, [(want_k[0], want_v[0])], 0.09, 0)
+    cache.truncate_front(0, 30)
+    assert np.array_equal(cache.gather(1, 30)[0].as_slice(), want_k[:, :, 18:])
+    cache.close()
+
+
 def test_refusals(device):
     fb = _fb()
     UN, SH, IN = fb._lib.UNSUPPORTED, fb._lib.SHAPE_MISMATCH, fb._lib.INVALID_ARGUMENT
