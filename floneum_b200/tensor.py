@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import math
+import struct
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -21,6 +22,7 @@ from . import _lib
 from .device import Device
 
 F32, BF16, F16, U32 = _lib.F32, _lib.BF16, _lib.F16, _lib.U32
+_pack4 = struct.Struct("=Qii8q").pack  # _lib.Tensor4
 _ITEMSIZE = {F32: 4, BF16: 2, F16: 2, U32: 4}
 
 
@@ -56,11 +58,15 @@ class Tensor:
         self._shape = tuple(map(int, shape))
         self.dtype = dtype
         if strides is None:
-            strides, acc = [0] * len(self._shape), 1
-            for i in range(len(strides) - 1, -1, -1):
-                strides[i] = acc
-                acc *= self._shape[i]
-            self.strides = tuple(strides)
+            if len(self._shape) == 4:
+                _, h, s, d = self._shape
+                self.strides = (h * s * d, s * d, d, 1)
+            else:
+                strides, acc = [0] * len(self._shape), 1
+                for i in range(len(strides) - 1, -1, -1):
+                    strides[i] = acc
+                    acc *= self._shape[i]
+                self.strides = tuple(strides)
         else:
             self.strides = tuple(map(int, strides))
         self._owner = owner  # keeps a borrowed allocation (e.g. a torch tensor) alive
@@ -149,13 +155,8 @@ class Tensor:
     # ------------------------------------------------------------------ C views
     def _c4(self) -> _lib.Tensor4:
         assert len(self._shape) == 4, f"expected a rank-4 tensor, got shape {self._shape}"
-        t = _lib.Tensor4()
-        t.data = self.ptr
-        t.dtype = self.dtype
-        for i in range(4):
-            t.shape[i] = self._shape[i]
-            t.stride[i] = self.strides[i]
-        return t
+        # (a third of the time of filling the fields one by one, for each tensor of each call)
+        return _lib.Tensor4.from_buffer_copy(_pack4(self.ptr, self.dtype, 0, *self._shape, *self.strides))
 
     def _c2(self) -> _lib.Tensor2:
         assert len(self._shape) == 2 and self.dtype == F32, "masks are rank-2 f32 tensors"

@@ -51,6 +51,16 @@ def test_a_cache_has_bf16_or_8_bit_pages():
             fb.KvCache.new(2, 64, dtype)
 
 
+def test_the_c_view_of_a_tensor():
+    fb = _fb()
+    from floneum_b200 import _lib
+    assert ctypes.sizeof(_lib.Tensor4) == 80
+    for t in (fb.Tensor(None, 2 ** 47 + 16, (2, 3, 5, 64), fb.BF16), fb.Tensor(None, 4096, (1, 2, 3, 4), fb.F32, (2 ** 40, 7, 0, 1))):
+        c = t._c4()
+        assert (c.data, c.dtype, tuple(c.shape), tuple(c.stride)) == (t.ptr, t.dtype, t.shape(), tuple(t.strides))
+    assert fb.Tensor(None, 0, (2, 3, 5, 64)).strides == (960, 320, 64, 1) and fb.Tensor(None, 0, (4, 3, 2)).strides == (6, 2, 1)
+
+
 def test_null_arguments_are_status_codes():
     from floneum_b200 import _lib
     L = _lib.load()
