@@ -78,8 +78,11 @@ __device__ __forceinline__ int place_row(const PlaceParams& P, int b, int t, int
 
 // ---------------------------------------------------------------------------------------------------------------
 // The vector form, for D a multiple of 16, tensors of one type and 16-byte aligned rows: a thread takes 16 elements of a row, 8 pairs with
-// their cos / sin values, and walks heads with them.  HBM-bound: several heads' loads are issued together, one thread per item.  The
-// D / 16 threads of a row are neighbours in a warp and find its largest element by shuffles.
+// their cos / sin values, and walks heads with them.  HBM-bound, so the loads of two query heads (or of a kv head's k and v) are issued
+// together and three blocks lie on an SM: with twice the loads a thread 128 registers leave two blocks, 24.8 against 24.6 us, and 26.7
+// without the cheaper maximum below; one warp per row took 345 us with the read-back, 52 now.  The D / 16 threads of a row are neighbours in
+// a warp and find its largest element by shuffles.  B4 H8 S4096 D128 bf16, k and v 24.6 us (4.1 TB/s, 3 of it the launch); with q of 32
+// heads rotated 67.6 us (5.5 TB/s); on three axes 68.9.
 template <int T>
 struct PlaceType {
     static constexpr int ES = T == 0 ? 4 : 2, U4 = ES / 2;  // bytes of an element; 16-byte vectors of 8 of them
@@ -167,6 +170,7 @@ __device__ __forceinline__ int place_codes(float (&a)[8], float (&z)[8], uint2 (
 // sequence, and a group of query heads or, from q_groups on, of kv heads.
 template <int PAGES, int ROT, int T, int D>
 __global__ void __launch_bounds__(256, 3) place_vec_kernel(const __grid_constant__ PlaceParams P, const unsigned q_groups, const unsigned per_thread) {
+    after_previous_launch();
     if (PAGES && blockIdx.y == 0) P.lens.publish();
     constexpr int U4 = PlaceType<T>::U4, U = T == 0 ? 1 : 2;  // query heads whose loads are in flight (of k and v: one head's)
     const int d = D ? D : P.D, half = d >> 1;
@@ -281,35 +285,52 @@ __global__ void __launch_bounds__(256) place_rows_kernel(const __grid_constant__
         const long long* st = is_q ? P.qs : is_k ? P.ks : P.vs;
         const long long src = b * st[0] + hk * st[1] + t * st[2];
         const bool turn = P.cos_t && (is_q || is_k);
-        auto value = [&](int d) {
-            const float a = ld_as_float(x, dtype, src + d);
-            if (!turn) return a;
-            const int i = P.interleaved ? d >> 1 : d % half, first = P.interleaved ? !(d & 1) : d < half;
-            const int partner = P.interleaved ? d ^ 1 : first ? d + half : d - half;
+        // the two values of pair i, at da and db; whoever reads them writes them, so a dense row may be rotated where it lies
+        const auto pair = [&](int i, int& da, int& db, float& ya, float& yb) {
+            da = P.interleaved ? 2 * i : i;
+            db = P.interleaved ? 2 * i + 1 : i + half;
+            ya = ld_as_float(x, dtype, src + da);
+            yb = ld_as_float(x, dtype, src + db);
+            if (!turn) return;
             const long long at = (long long)place_row(P, b, t, i) * half + i;
-            const float z = ld_as_float(x, dtype, src + partner), c = __ldg(P.cos_t + at), s = __ldg(P.sin_t + at);
-            float ya, yb;
-            rope_pair(first ? a : z, first ? z : a, c, s, P.interleaved, ya, yb);
-            return first ? ya : yb;
+            rope_pair(ya, yb, __ldg(P.cos_t + at), __ldg(P.sin_t + at), P.interleaved, ya, yb);
         };
+        int da, db;
+        float ya, yb;
         if (is_q || !P.pages) {
             const long long* os = is_q ? P.qos : P.vs;
             const long long dst = b * os[0] + hk * os[1] + t * os[2];
-            for (int d = lane; d < P.D; d += 32) st_from_float(is_q ? P.q_out : P.k_pages, is_q ? P.qo_dtype : P.v_dtype, dst + d, value(d));
+            for (int i = lane; i < half; i += 32) {
+                pair(i, da, db, ya, yb);
+                st_from_float(is_q ? P.q_out : P.k_pages, is_q ? P.qo_dtype : P.v_dtype, dst + da, ya);
+                st_from_float(is_q ? P.q_out : P.k_pages, is_q ? P.qo_dtype : P.v_dtype, dst + db, yb);
+            }
             continue;
         }
         const int at = P.lens.before(b) + t;
         const long long tile = (long long)P.page_table[(long long)b * P.max_pages + at / DEC_PT] * P.Hkv + hk;
         const long long dst = (tile * DEC_PT + at % DEC_PT) * P.D;
         if (P.pages == 1) {
-            for (int d = lane; d < P.D; d += 32) static_cast<__nv_bfloat16*>(is_k ? P.k_pages : P.v_pages)[dst + d] = __float2bfloat16_rn(value(d));
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_k ? P.k_pages : P.v_pages) + dst;
+            for (int i = lane; i < half; i += 32) {
+                pair(i, da, db, ya, yb);
+                out[da] = __float2bfloat16_rn(ya);
+                out[db] = __float2bfloat16_rn(yb);
+            }
             continue;
         }
         uint32_t top = 0;
-        for (int d = lane; d < P.D; d += 32) top = max(top, abs_bits(value(d)));
+        for (int i = lane; i < half; i += 32) {
+            pair(i, da, db, ya, yb);
+            top = max(top, max(abs_bits(ya), abs_bits(yb)));
+        }
         const int byte = row8_byte(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
-        for (int d = lane; d < P.D; d += 32)
-            static_cast<int8_t*>(is_k ? P.k_pages : P.v_pages)[dst + d] = byte == kRowNaN ? 0 : (int8_t)row8_code(value(d), row8_inverse(byte));
+        int8_t* out = static_cast<int8_t*>(is_k ? P.k_pages : P.v_pages) + dst;
+        for (int i = lane; i < half; i += 32) {
+            pair(i, da, db, ya, yb);
+            out[da] = byte == kRowNaN ? 0 : (int8_t)row8_code(ya, row8_inverse(byte));
+            out[db] = byte == kRowNaN ? 0 : (int8_t)row8_code(yb, row8_inverse(byte));
+        }
         if (lane == 0) P.scales[(tile * 2 + (is_k ? 0 : 1)) * DEC_PT + at % DEC_PT] = (uint8_t)byte;
     }
 }
@@ -344,10 +365,13 @@ __device__ __forceinline__ void row8_values(uint32_t codes, float step, float* f
 }
 
 // A warp takes a page of K, then of V, all its loads at once, eight elements (16-bit pages) or sixteen (8-bit) per lane.  T: type of the
-// results, whose rows start on multiples of 16 bytes, or 3: any types, any rows.  blockIdx.y: (sequence, kv head).
+// results, whose rows start on multiples of 16 bytes, or 3: any types, any rows.  blockIdx.y: (sequence, kv head).  Half bound by HBM, half
+// by the instructions that make values of codes (3 per element): B4 H8 S4096 D128 8-bit pages to bf16 (33 MB read, 67 written) 20.1 us =
+// 5 TB/s; K and V together with 80 registers and two blocks an SM 21.1, a thread per 16 codes 22.9.
 template <int PAGES, int D, int T>
 __global__ void __launch_bounds__(256, 4) kvcache_gather_page_kernel(const __grid_constant__ GatherPageParams P) {
     constexpr int E = PAGES == 2 ? 16 : 8, CH = D / E, ROWS = 32 / CH, N = DEC_PT / ROWS;  // elements of a lane, lanes of a row, rows at once, rounds
+    after_previous_launch();
     const int lane = threadIdx.x & 31, c = lane % CH * E, row = lane / CH;
     for (int pair = blockIdx.y; pair < P.B * P.Hkv; pair += gridDim.y) {
         const int b = pair / P.Hkv, hk = pair % P.Hkv, front = __ldg(P.front + b), end = __ldg(P.end + b);

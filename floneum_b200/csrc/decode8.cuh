@@ -629,6 +629,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     __shared__ int n_complete;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cta0 = (int)blockIdx.x * D8_NW, share = cta0 + warp;
+    after_previous_launch();
     // T pages in all
     int sum = 0;
     for (int b0 = 0; b0 < P.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < P.B ? (P.end[b0 + lane] + DEC_PT - 1) / DEC_PT : 0);
@@ -760,6 +761,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
     float2* push_ml = reinterpret_cast<float2*>(push + Decode8ClusterSmem<D>::SLOT_F4);    // [source CTA][GP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = C > 1 ? (int)cluster_cta_rank() : 0;
+    after_previous_launch();
     const int head = (int)blockIdx.x / C, b = head / P.Hkv, hk = head % P.Hkv;
     const int end = __ldg(P.end + b), front = __ldg(P.front + b), pages = (end + DEC_PT - 1) / DEC_PT;
     const int p_begin = (int)((long long)pages * rank / C), n = (int)((long long)pages * (rank + 1) / C) - p_begin;

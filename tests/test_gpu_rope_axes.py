@@ -184,6 +184,29 @@ def test_a_window_that_a_prompt_overruns(device):
         assert np.array_equal(ck.as_slice(), keep(_turn(k, cos, sin, ids, axes, False)[:, :, -w:])) and np.array_equal(cv.as_slice(), keep(v[:, :, -w:]))
 
 
+@pytest.mark.parametrize("D,off", [(128, 0), (80, 0), (64, 1), (6, 0)])
+def test_a_tensor_rotated_where_it_lies(device, D, off):
+    import ctypes
+    import torch
+    fb = _fb()
+    from floneum_b200.rope import _positions
+    rng = np.random.default_rng(D + off)
+    cos, sin = (rng.uniform(-1, 1, (40, D // 2)).astype(np.float32) for _ in range(2))
+    tc, ts = _T(device, cos), _T(device, sin)
+    ids, axes = rng.integers(0, 40, (2, 2, 21)).astype(np.uint32), fb.axes_of_sections([D // 4, D // 2 - D // 4])
+    for interleaved in (0, 1):
+        wide = torch.tensor(rng.standard_normal((2, 3, 21, D + 8)).astype(np.float32)).cuda()
+        x = wide[..., off:off + D]
+        before = x.cpu().numpy().copy()
+        torch.cuda.synchronize()
+        tid = _T(device, ids, fb.U32)
+        pos, cx = _positions(tid, axes, 2, 21, D), fb.Tensor.from_torch(device, x)._c4()
+        fb._lib.check(fb._lib.load().fusor_cuda_rope_axes(device.handle, ctypes.byref(cx), tc.ptr, ts.ptr, 40, ctypes.byref(pos), interleaved,
+                                                          ctypes.byref(cx)), device.handle)
+        device.synchronize()
+        assert np.array_equal(x.cpu().numpy(), _turn(before, cos, sin, ids, axes, interleaved))
+
+
 def test_a_position_outside_the_tables_is_reported(device):
     """Read as row 0 and reported at the next wait; the context stays usable."""
     fb = _fb()
