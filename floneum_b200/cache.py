@@ -238,7 +238,8 @@ class PagedKvCache:
         return k, v
 
     def set_decode_ctas(self, ctas: int):
-        """Grid size of the decode kernel: 0 = automatic (from the number of cached pages), n > 0 = exactly n CTAs."""
+        """Grid size of the decode kernel: 0 = automatic (from the number of cached pages), n > 0 = exactly n CTAs (up to four per SM;
+        8-bit pages: one)."""
         self._ck(self._L.fusor_cuda_kvcache_set_decode_ctas(self._h, int(ctas)))
 
     def decode(self, q: Tensor, scale: float, out: Optional[Tensor] = None, out_dtype: int = F32) -> Tensor:

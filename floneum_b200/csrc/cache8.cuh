@@ -81,8 +81,8 @@ __device__ __forceinline__ int place_row(const PlaceParams& P, int b, int t, int
 // their cos / sin values, and walks heads with them.  HBM-bound, so the loads of two query heads (or of a kv head's k and v) are issued
 // together and three blocks lie on an SM: with twice the loads a thread 128 registers leave two blocks, 24.8 against 24.6 us, and 26.7
 // without the cheaper maximum below; one warp per row took 345 us with the read-back, 52 now.  The D / 16 threads of a row are neighbours in
-// a warp and find its largest element by shuffles.  B4 H8 S4096 D128 bf16, k and v 24.6 us (4.1 TB/s, 3 of it the launch); with q of 32
-// heads rotated 67.6 us (5.5 TB/s); on three axes 68.9.
+// a warp and find its largest element by shuffles.  B4 H8 S4096 D128 bf16, k and v 24.8 us (4.1 TB/s); with q of 32 heads rotated 64.4;
+// on three axes 66.0 (graphs).
 template <int T>
 struct PlaceType {
     static constexpr int ES = T == 0 ? 4 : 2, U4 = ES / 2;  // bytes of an element; 16-byte vectors of 8 of them

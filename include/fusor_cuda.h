@@ -281,13 +281,14 @@ int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* cache, const fusor_cuda_te
 /* ------------------------------------------------------------------------------------------------
  * Decode: one query token per sequence against the paged cache (the Sq == 1 regime of the call site,
  * models/kalosm-llama/src/raw/attention_layer.rs:405-448; all-zero mask [1, kv_len]).
- *   q [B,Hq,1,D] (bf16, f16 or f32; rounded to bf16, the type of the cached keys), out [B,Hq,1,D] (f32, bf16 or f16;
- *   rows start on a multiple of four elements).
+ *   q [B,Hq,1,D] (bf16, f16 or f32; rounded to bf16, the type of the cached keys; an 8-bit cache takes f32 queries to 22 bits of the
+ *   head's largest element), out [B,Hq,1,D] (f32, bf16 or f16; rows start on a multiple of four elements).
  * Up to as many (sequence, kv head) pairs as SMs, with a longest sequence from 8 pages to a few thousand tokens: one launch, a
  * cluster of CTAs per pair.  Else split-KV: the pages of all (sequence, kv head) pairs are dealt evenly to a persistent grid by the kernel itself, from
  * the lengths on the device (a step after an append plans and uploads nothing on the host); each CTA emits a partial
  * (m, l, O) per run of pages, and a second kernel, which finds each head's partials with the same deal, merges them by
- * log-sum-exp. */
+ * log-sum-exp (over 8-bit pages the CTA that completes a pair merges its partials: one launch).  Work of one cache shares its partials:
+ * captured graphs that hold decodes of one cache must not run at the same time. */
 int32_t fusor_cuda_flash_attention_decode(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* q,
                                           float scale, const fusor_cuda_tensor4* out);
 /* Same, but leaves the result un-normalised for a merge across GPUs that each hold a chunk of the keys:
@@ -298,7 +299,8 @@ int32_t fusor_cuda_flash_attention_decode(fusor_cuda_ctx* ctx, fusor_cuda_kvcach
 int32_t fusor_cuda_flash_attention_decode_partial(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* cache,
                                                   const fusor_cuda_tensor4* q, float scale, float* partial);
 /* Grid size of the decode kernel: 0 (default) = chosen from the number of cached pages, in whole multiples of the SM
- * count; n > 0 = exactly n CTAs (tuning; the reference has no counterpart, its kernel has one workgroup per row). */
+ * count; n > 0 = exactly n CTAs, up to four per SM, of an 8-bit cache one (tuning; the reference has no counterpart, its kernel has
+ * one workgroup per row). */
 int32_t fusor_cuda_kvcache_set_decode_ctas(fusor_cuda_kvcache* cache, int32_t ctas);
 /* ------------------------------------------------------------------------------------------------
  * Exchange of split-KV records between the GPUs of one node over peer memory (no counterpart in the reference, which
