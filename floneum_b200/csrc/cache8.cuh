@@ -79,8 +79,8 @@ __device__ __forceinline__ int place_row(const PlaceParams& P, int b, int t, int
 // ---------------------------------------------------------------------------------------------------------------
 // The vector form, for D a multiple of 16, tensors of one type and 16-byte aligned rows: a thread takes 16 elements of a row, 8 pairs with
 // their cos / sin values, and walks heads with them.  HBM-bound, so the loads of two query heads (or of a kv head's k and v) are issued
-// together and three blocks lie on an SM: with twice the loads a thread 128 registers leave two blocks, 24.8 against 24.6 us, and 26.7
-// without the cheaper maximum below; one warp per row took 345 us with the read-back, 52 now.  The D / 16 threads of a row are neighbours in
+// together and three blocks lie on an SM: with twice the loads a thread 128 registers leave two blocks, 24.8 against 24.6 us
+// (each then a launch of its own), and 26.7 without the cheaper maximum below; one warp per row took 345 us with the read-back, 52 now.  The D / 16 threads of a row are neighbours in
 // a warp and find its largest element by shuffles.  B4 H8 S4096 D128 bf16, k and v 24.8 us (4.1 TB/s); with q of 32 heads rotated 64.4;
 // on three axes 66.0 (graphs).
 template <int T>
@@ -93,7 +93,7 @@ template <int T>
 __device__ __forceinline__ void place_fetch(const void* base, long long at, uint4 (&raw)[PlaceType<T>::U4]) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at * PlaceType<T>::ES);
 #pragma unroll
-    for (int j = 0; j < PlaceType<T>::U4; ++j) raw[j] = __ldcs(p + j);
+    for (int j = 0; j < PlaceType<T>::U4; ++j) raw[j] = ld_stream(p + j);
 }
 template <int T>
 __device__ __forceinline__ void place_floats(const uint4 (&raw)[PlaceType<T>::U4], float (&f)[8]) {
@@ -374,18 +374,18 @@ __global__ void __launch_bounds__(256, 4) kvcache_gather_page_kernel(const __gri
     after_previous_launch();
     const int lane = threadIdx.x & 31, c = lane % CH * E, row = lane / CH;
     for (int pair = blockIdx.y; pair < P.B * P.Hkv; pair += gridDim.y) {
-        const int b = pair / P.Hkv, hk = pair % P.Hkv, front = __ldg(P.front + b), end = __ldg(P.end + b);
+        const int b = pair / P.Hkv, hk = pair % P.Hkv, front = P.front[b], end = P.end[b];
         const int pages = (front + P.len + DEC_PT - 1) / DEC_PT;
         for (int p = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5); p < pages; p += (int)((gridDim.x * blockDim.x) >> 5)) {
             const bool any = p * DEC_PT < end;
-            const long long tile = any ? (long long)__ldg(P.page_table + (long long)b * P.max_pages + p) * P.Hkv + hk : 0;
-            const float step = any && PAGES == 2 ? row8_step(__ldg(P.scales + tile * 2 * DEC_PT + lane)) : 0.0f;
+            const long long tile = any ? (long long)P.page_table[(long long)b * P.max_pages + p] * P.Hkv + hk : 0;
+            const float step = any && PAGES == 2 ? row8_step(P.scales[tile * 2 * DEC_PT + lane]) : 0.0f;
             const auto rows = [&](int which, auto big) {
                 uint4 raw[N] = {};
                 if (any) {
                     const uint4* from = reinterpret_cast<const uint4*>(which ? P.v_pages : P.k_pages) + tile * (DEC_PT * D / E) + lane;
 #pragma unroll
-                    for (int j = 0; j < N; ++j) raw[j] = __ldcs(from + j * 32);
+                    for (int j = 0; j < N; ++j) raw[j] = ld_stream(from + j * 32);
                 }
                 const long long* st = which ? P.vs : P.ks;
                 const int dtype = T < 3 ? T : which ? P.v_dtype : P.k_dtype;

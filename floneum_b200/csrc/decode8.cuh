@@ -106,7 +106,7 @@ struct Decode8Walk {
         hk = 0;
         do {
             ++b;
-            np = (__ldg(P.end + b) + DEC_PT - 1) / DEC_PT;
+            np = (P.end[b] + DEC_PT - 1) / DEC_PT;
         } while (np == 0);
     }
 };
@@ -129,7 +129,7 @@ struct Decode8Feed {
             seek(P);
         }
         hk[k] = w.hk;
-        page[k] = __ldg(entry);  // first used by its copy
+        page[k] = *entry;  // first used by its copy
         entry += step;
         i += step;
     }
@@ -219,10 +219,10 @@ __device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk,
             const long long at = b * P.q_sb + (long long)(hk * P.g + h) * P.q_sh + 4 * word;
             if (P.q_dtype == 0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) raw[u][e] = __ldg(static_cast<const uint32_t*>(P.q) + at + e);
+                for (int e = 0; e < 4; ++e) raw[u][e] = static_cast<const uint32_t*>(P.q)[at + e];
             } else {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) raw[u][e] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(P.q) + at) + e);
+                for (int e = 0; e < 2; ++e) raw[u][e] = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(P.q) + at)[e];
             }
         }
 #pragma unroll
@@ -573,7 +573,7 @@ struct Decode8Records {
 // of eight records do not wait for their weights.
 template <int D>
 __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const Decode8Records& R, int pair, int rr, int lane) {
-        constexpr int E = D / 32, BATCH = 8;
+    constexpr int E = D / 32, BATCH = 8;
     const int b = pair / P.Hkv, hk = pair % P.Hkv;
     float M = -INFINITY, L = 0.0f, acc[E] = {};
     for (int i0 = 0; i0 < R.n; i0 += BATCH) {
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     int open = -1;
     for (int i = 0; i < n; w.next(P)) {
         const int seg_end = min(n, w.off + w.np);
-        const int front = __ldg(P.front + w.b), len = __ldg(P.end + w.b) - front;
+        const int front = P.front[w.b], len = P.end[w.b] - front;
         uint32_t* digits = reinterpret_cast<uint32_t*>(d8_smem + warp * Smem::WARP + ring.spare);
         __syncwarp();  // every lane is done with the slot
         d8_digits<D>(P, w.b, w.hk, 0, 1, digits, lane);
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
     const int rank = C > 1 ? (int)cluster_cta_rank() : 0;
     after_previous_launch();
     const int head = (int)blockIdx.x / C, b = head / P.Hkv, hk = head % P.Hkv;
-    const int end = __ldg(P.end + b), front = __ldg(P.front + b), pages = (end + DEC_PT - 1) / DEC_PT;
+    const int end = P.end[b], front = P.front[b], pages = (end + DEC_PT - 1) / DEC_PT;
     const int p_begin = (int)((long long)pages * rank / C), n = (int)((long long)pages * (rank + 1) / C) - p_begin;
     if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before the first push
 

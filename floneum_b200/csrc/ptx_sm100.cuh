@@ -24,6 +24,13 @@ __device__ __forceinline__ void after_previous_launch() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// A streaming load that stays behind after_previous_launch().  What the launch before may have written is read by this or by plain loads:
+// __ldg and __ldcs tell the compiler that nobody writes the data, so it may read them before the wait.
+__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+    uint4 x;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+    return x;
+}
 
 // ----------------------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

@@ -475,6 +475,34 @@ def test_one_cache_at_one_grid_after_another(device):
         del graph
 
 
+@pytest.mark.parametrize("B,past", [(1, 3), (2, 40), (40, 100)])
+def test_each_launch_sees_what_the_one_before_wrote(device, B, past):
+    """Rows rotated and written, attended over and read back, with nothing between the launches: what comes of it when each is waited for.
+    40 sequences: their lengths come from the device's tables, and do not travel with the launch."""
+    fb = _fb()
+    rng = np.random.default_rng(B)
+    steps, Hq, Hkv, D = 24, 8, 2, 128
+    x = [rng.standard_normal((B, h, past + steps, D)).astype(np.float32) for h in (Hq, Hkv, Hkv)]
+
+    def run(wait):
+        rope, cache, outs = fb.RopeCache.new(D, past + steps, 10000.0, device), _cache(device, B, Hkv, D, past + steps), []
+        parts = [[_T(device, np.ascontiguousarray(t[:, :, at:end])) for t in x] for at, end in [(0, past)] + [(past + i, past + i + 1) for i in range(steps)]]
+        for i, (q, k, v) in enumerate(parts):
+            q = rope.forward_append(q, k, v, cache)
+            wait()
+            if i:
+                outs.append(cache.decode(q, 0.09))
+                wait()
+            outs += cache.gather(B, past + i, 1)
+            wait()
+        return [t.as_slice() for t in outs]
+
+    alone = run(device.synchronize)
+    for _ in range(3):
+        for got, want in zip(run(lambda: None), alone):
+            assert np.array_equal(got, want)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
 def test_any_scale_and_a_query_of_zeros(device, scale):
     rng = np.random.default_rng(2)
