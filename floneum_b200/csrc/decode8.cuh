@@ -642,11 +642,15 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     int sum = 0;
     for (int b0 = 0; b0 < P.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < P.B ? (P.end[b0 + lane] + DEC_PT - 1) / DEC_PT : 0);
     const int T = sum * P.Hkv;
-    const Decode8Deal deal(T, shares);
+    // `shares` is from the launch.  A captured one may meet shorter sequences: as many shares as pages then, since Decode8Records looks for
+    // a record in the first share of a CTA.  (In mode 2 the merge goes by the launch's number; shares with no page write empty records.)
+    const bool merged_later = P.res.mode == 2;
+    const Decode8Deal deal(T, merged_later ? shares : max(1, min(shares, T)));
     const int first = deal.bound(share), n = deal.bound(share + 1) - first;  // (a share has a page at least; warps past the last: none)
     // the sequence that holds the warp's first page, and the pages (per kv head) before it
     Decode8Walk w{};
-    for (int b0 = 0, cum = 0; n > 0; b0 += 32) {
+    const bool nothing = merged_later && n == 0 && share < shares && first < T;
+    for (int b0 = 0, cum = 0; n > 0 || nothing; b0 += 32) {
         const int pages = b0 + lane < P.B ? (P.end[b0 + lane] + DEC_PT - 1) / DEC_PT : 0;
         int upto = pages;
 #pragma unroll
@@ -666,6 +670,8 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
         }
         cum += __shfl_sync(0xffffffffu, upto, 31);
     }
+    if (nothing && lane < P.g)
+        *reinterpret_cast<float2*>(P.part_ml + ((long long)(w.b * P.Hkv + w.hk + share) * DEC_GP + lane) * 2) = make_float2(-INFINITY, 0.0f);
     Decode8Ring<D> ring(d8_smem, warp, lane);
     Decode8Feed feed;
     feed.init(P, w, 0, n, 1);

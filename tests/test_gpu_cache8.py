@@ -224,6 +224,7 @@ def _filled(device, rng, lens, Hkv, D, k_scale=1.0, v_scale=1.0):
         x = values(codes, bytes_)[table[b, :pages[b]]]
         return x.transpose(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :lens[b]]
 
+    cache.table = table
     return cache, [(dense(kc, kb, b), dense(vc, vb, b)) for b in range(len(lens))]
 
 
@@ -501,6 +502,46 @@ def test_each_launch_sees_what_the_one_before_wrote(device, B, past):
     for _ in range(3):
         for got, want in zip(run(lambda: None), alone):
             assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("exchange", [False, True])
+def test_a_captured_decode_meets_other_lengths(device, D, exchange):
+    """Captured at one set of lengths, replayed at shorter ones (fewer pages than warps, to a page in all) and at the first ones again."""
+    import torch
+    fb = _fb()
+    from floneum_b200.sharding import PeerExchange
+    stream = torch.cuda.Stream()
+    dev = fb.Device.gpu(0, stream.cuda_stream)
+    rng = np.random.default_rng(D)
+    lens = [6000, 33, 2500]
+    cache, rows = _filled(dev, rng, lens, 2, D)
+    cache.set_decode_ctas(148)  # not the cluster
+    q = rng.standard_normal((3, 8, 1, D)).astype(np.float32)
+    tq = _T(dev, q)
+    ex = PeerExchange(dev, 0, 1, 3 * 8 * (D + 2)) if exchange else None
+    there = torch.zeros((3, 8, D) if exchange else q.shape, device="cuda")
+    torch.cuda.synchronize()
+    out = fb.Tensor.from_torch(dev, there)
+    decode = (lambda: ex.decode(cache, tq, 0.09, out)) if exchange else (lambda: cache.decode(tq, 0.09, out=out))
+    decode()
+    dev.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+        decode()
+    for now in ([6000, 33, 2500], [400, 33, 100], [17, 1, 16], [6000, 1, 40], [1, 33, 1], [6000, 33, 2500]):
+        cache.set_page_table(cache.table, np.asarray(now, np.int32))
+        decode()  # the tables to the device
+        dev.synchronize()
+        there.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = there.cpu().numpy()
+        _check(got[:, :, None] if exchange else got, q, [tuple(x[:, :n] for x in r) for r, n in zip(rows, now)], 0.09, 0)
+    del graph
+    if ex:
+        ex.close()
 
 
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
