@@ -379,6 +379,12 @@ class KvCache:
         if start_pos < 0:
             start_pos = self.current_seq_len()
         n = k.shape()[2]
+        if positions is not None or axes is not None:  # before any row gives way
+            from .rope import _positions
+            assert positions is not None and axes is not None, "positions and axes come together"
+            assert q.shape()[0] == k.shape()[0] and q.shape()[2:] == k.shape()[2:], f"q {list(q.shape())} and k {list(k.shape())} differ in batch, tokens or head_dim"
+            if self.current_seq_len() + n > self.max_sequence_len:
+                _positions(positions, axes, k.shape()[0], n, k.shape()[3])
         k2, v2, skip = self._make_room(q.device, k, v)
         if skip:  # the rows that do not survive still rotate q; do that with the plain op and append the rest
             from .rope import rope, rope_axes

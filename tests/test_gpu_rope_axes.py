@@ -283,3 +283,22 @@ def test_refusals(device):
                             axes=np.zeros(32, np.uint8))
     assert cache.seq_len(0) == 0
     device.synchronize()
+
+
+def test_a_refused_append_leaves_a_full_window_as_it_was(device):
+    """Positions that do not fit are refused before the oldest rows give way to the new ones."""
+    fb = _fb()
+    rng = np.random.default_rng(8)
+    rope, axes = fb.RopeCache.new(64, 64, 10000.0, device), fb.axes_of_sections([16, 16])
+    x = lambda n, h=2: _T(device, rng.standard_normal((1, h, n, 64)).astype(np.float32))
+    ids = lambda n, a=2: _T(device, np.zeros((a, n), np.uint32), fb.U32)
+    cache = fb.KvCache(2, 20, dtype=fb.I8)
+    cache.append(device, x(20), x(20))
+    before = [t.copy() for t in (lambda s: (s["k"], s["v"]))(cache.export_session())]
+    for kw in (dict(positions=ids(4), axes=axes), dict(positions=ids(3), axes=axes[:-1]), dict(positions=ids(3)), dict(axes=axes)):
+        with pytest.raises(AssertionError):
+            rope.forward_append(x(3, 4), x(3), x(3), cache, **kw)
+    with pytest.raises(AssertionError):
+        rope.forward_append(x(2, 4), x(3), x(3), cache, positions=ids(3), axes=axes)
+    after = cache.export_session()
+    assert all(np.array_equal(a, after[name]) for a, name in zip(before, ("k", "v")))
