@@ -18,7 +18,7 @@
 // B64 kv 1024-8192 H32/8 D128, 610 MB: 110 to 112 us in graphs = 5.5 TB/s; the bf16 cache's kernels take 193 us for these sequences.  Time stamps:
 // dealt 1.5 us, first copies 4, first page used 6.5; pages done on average at 90, the last at 100; the last CTA ends at 108.  610 MB in
 // those 84 us are 7.2 TB/s: HBM is the bound in between, and the ends are latencies and the spread of the warps, which a deal at run
-// time would even out at the price of results that depend on it.  394 warp instructions a page with all ends (ALU 43 % busy, the tensor
+// time would even out at the price of results that depend on it.  401 warp instructions a page with all ends (ALU 45 % busy, the tensor
 // pipe 32 %).  16-bit MMAs on converted keys took 519 a page and 130 us, 8-bit ones before each warp had a run of pages 135, with it and a
 // second launch for the merge 118.
 #pragma once
