@@ -15,7 +15,8 @@
 // The references (of the sum and of the output) follow the maxima lazily: a page whose scores exceed them by less than 2^8 leaves them.
 // Error of an f32 result against 64 bits: 2.4e-7 to 3.5e-7 (2-norm), that of f32 arithmetic in torch 4.5e-7 to 1.1e-6.
 //
-// B64 kv 1024-8192 H32/8 D128, 610 MB: 110 to 112 us in graphs = 5.5 TB/s; the bf16 cache's kernels take 193 us for these sequences.  Time stamps:
+// B64 kv 1024-8192 H32/8 D128, 610 MB: 110 to 112 us in graphs = 5.5 TB/s; the bf16 cache's kernels take 193 us for these sequences.  Time stamps (without the overlap with the
+// launch before):
 // dealt 1.5 us, first copies 4, first page used 6.5; pages done on average at 90, the last at 100; the last CTA ends at 108.  610 MB in
 // those 84 us are 7.2 TB/s: HBM is the bound in between, and the ends are latencies and the spread of the warps, which a deal at run
 // time would even out at the price of results that depend on it.  401 warp instructions a page with all ends (ALU 45 % busy, the tensor
@@ -758,9 +759,9 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
 }
 
 // Few pages: a cluster of C CTAs per (sequence, kv head), as decode_cluster_kernel: one launch, the CTAs' states meet in shared
-// memory over the cluster.  Bound by latencies: of 6.6 us for 1411 tokens (H32/8 D128, medians of time stamps, without the launch) 1.4 go to the
-// lengths, 0.5 to the page table, 0.6 to the query's digits, 1.4 to the pages, 1.4 to the CTA's merge, 1.2 to the cluster's.  With the
-// launch 7.6, where the bf16 cache takes 6.4: so few pages gain nothing from being half as long.
+// memory over the cluster.  Bound by latencies: of 6.6 us for 1411 tokens (H32/8 D128, medians of time stamps, without the overlap with the launch before) 1.4 go to the
+// lengths, 0.5 to the page table, 0.6 to the query's digits, 1.4 to the pages, 1.4 to the CTA's merge, 1.2 to the cluster's.  Back to back in
+// graphs 7.5 to 7.6, where the bf16 cache takes 6.4: so few pages gain nothing from being half as long.
 template <int D>
 struct Decode8ClusterSmem {
     static constexpr int SLOT_F4 = DEC_GP * D / 4 + DCL_MAX;  // column groups pushed here by all CTAs (rounded up per source)

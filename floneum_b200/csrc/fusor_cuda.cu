@@ -1951,12 +1951,13 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
     for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
     const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;  // bytes of a page pair
     // CTAs of the even deal: a record per CTA and pair, which one CTA merges, so not more than 32 to a pair (one sequence of 64000
-    // tokens with one kv head: 45 us from 148 CTAs, 27 from 32)
+    // tokens with one kv head: 38.7 us from 148 CTAs, 25.7 from 32)
     const int grid = c->decode_ctas > 0 ? c->decode_ctas : (int)std::min<long long>(ctx->num_sms, 32 * heads);
     // A cluster per (sequence, kv head), of the largest size of which all fit at once, while its longest share is short enough.  Measured
     // (ns, 4 KB page pairs): the cluster 7200 + 93 per page of that share, the deal 13000 + 98 per page of a CTA's.  One sequence of
-    // 1411 tokens 7.9 against 12.2 us, of 12000 15.9 and 19.1, of 24000 23.1 and 22.4; four of 8192 19.5 and 22.5; sixteen of 256 .. 4096
-    // 28.1 and 25.1 (32 query heads on 8 of 128, graphs, pages cold).
+    // 1411 tokens 7.5 against 11.5 us, of 12000 15.3 and 18.0; four of 8192 18.8 and 21.8; sixteen of 2048 18.5 and 23.2 (32 query heads
+    // on 8 of 128, graphs, pages cold).  Where the deal is taken, without the overlap with the launch before: one of 24000 23.1 and
+    // 22.4 (with it the deal 21.3), sixteen of 256 .. 4096 28.1 and 25.1 (25.4).  The rule's numbers are from those runs too.
     if (P.res.mode != 2 && c->decode_ctas == 0 && heads <= ctx->num_sms && longest >= 1) {
         int i = 0;
         while (i < 3 && heads <= ctx->clusters[i + 1]) ++i;
