@@ -606,8 +606,9 @@ __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const D
         for (int e = 0; e < E; ++e) acc[e] *= before;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-            const float a = __shfl_sync(0xffffffffu, weight, k);
-            if (k < here && a != 0.0f) {
+            // (a weight that is zero next to the largest score keeps a record's NaN; only a record without keys counts for nothing)
+            const float a = __shfl_sync(0xffffffffu, weight, k), sum = __shfl_sync(0xffffffffu, x.y, k);
+            if (k < here && sum != 0.0f) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] += a * o[k][e];
             }
