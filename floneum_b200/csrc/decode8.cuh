@@ -680,12 +680,12 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     if (n > 0) d8_prefetch_q<D>(P, w.b, w.hk, lane);
     ring.fill(P, feed, lane);
 
-    if (P.res.mode == 1)  // sequences without pages: empty records
+    if (P.res.mode != 2)  // sequences without pages (mode 0: in a replay only): empty records, zeros
         for (int row = (int)blockIdx.x * D8_THREADS + tid; row < P.B * P.res.Hq; row += gridDim.x * D8_THREADS)
             if (P.end[row / P.res.Hq] == 0) {
-                float* r = static_cast<float*>(P.res.out) + (long long)row * (D + 2);
-                r[0] = -INFINITY;
-                for (int d = 1; d < D + 2; ++d) r[d] = 0.0f;
+                const int b = row / P.res.Hq, h = row % P.res.Hq;
+                for (int dg = 0; dg < D / 4; ++dg)
+                    decode_emit(P.res, D, P.g, b, h / P.g, h % P.g, dg, -INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
             }
     if (tid == 0) n_complete = 0;
     if (lane < 2) parts[2 * warp + lane] = make_int4(0, 0, 0, 0);
