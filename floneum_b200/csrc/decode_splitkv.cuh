@@ -847,7 +847,7 @@ __global__ void lse_combine_kernel(const float* parts, int n_parts, long long n_
             const float* pr = parts + ((long long)p * n_rows + row) * rec;
             if (pr[1] != 0.0f) acc += pr[2 + d] * __expf(pr[0] - M);
         }
-        out[row * D + d] = L > 0.0f ? acc / L : 0.0f;
+        out[row * D + d] = L == 0.0f ? 0.0f : acc / L;  // (a NaN of a sum stays one)
     }
 }
 

@@ -102,7 +102,7 @@ __device__ __forceinline__ void peer_merge_row(const float* slots, size_t slot_f
         const float* pr = base + (size_t)p * slot_floats;
         if (__ldcg(pr + 1) != 0.0f) L += __ldcg(pr + 1) * __expf(__ldcg(pr) - M);
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // (a NaN of a sum stays one)
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float acc = 0.0f;
         for (int p = 0; p < world; ++p) {
