@@ -6,7 +6,9 @@
 // MMAs whose rows are tokens (S^T = K Q^T) and dims (O^T = V^T P^T), so the eight columns are the query heads and none of
 // the 16 rows is padding.  Against f32 arithmetic on the values nothing is given up that the result would show:
 //  * scores are 8-bit MMAs on the codes as they lie: q, times a power of two per head, is a whole number of 22 to 23 bits, three digits
-//    of base 256, whose products with the codes are summed exactly; a score is scaled by its row's step in f32;
+//    of base 256, whose products with the codes are summed exactly; a score is scaled by its row's step in f32.  f32 queries have three
+//    digits more for what is left, 45 bits together; of 16-bit ones an element below 2^-14 (f16: 2^-11) of its head's largest is off by up to
+//    2^-23 of that;
 //  * the weight of a value row is exp(s) 2^ve in one exponential, against a running reference of its own, so that rows whose steps
 //    lie far apart weigh in f16 as they do in the result: a factor of 2^6 and two terms, 22 bits down to 2^-31 of the reference.
 //    The value codes become f16 by setting the exponent of 1024 over the byte and subtracting: exact;
@@ -30,9 +32,8 @@
 
 namespace fusor {
 
-constexpr int D8_NW = 16;     // warps of a CTA
+constexpr int D8_NW = 16;     // warps of a CTA (most)
 constexpr int D8_SLOTS = 3;   // pages of a warp: one in use, two on their way
-constexpr int D8_THREADS = D8_NW * 32;
 constexpr float D8_SHIFT = 6.0f;  // log2 of the factor the weights of value rows carry: with a page 2^8 above its reference 2^14
 
 struct Decode8Params {
@@ -55,14 +56,19 @@ struct Decode8Params {
     DecodeOutput res;
 };
 
-template <int D>
+// LEVELS: of the query's digits, 2 for f32 queries, 1 for 16-bit ones.  At D = 128 those take 24 registers more: fewer warps, with 168 each
+// instead of 128.
+template <int D, int LEVELS>
+constexpr int d8_warps = LEVELS > 1 && D == 128 ? 12 : D8_NW;
+
+template <int D, int NW = D8_NW>
 struct Decode8Smem {
     static constexpr int TILE = DEC_PT * D;      // bytes of a page's K or V codes
     static constexpr int SLOT = 2 * TILE + 128;  // K, V, 32 scales and padding: rows of K and V start on multiples of 64 or 128
     static constexpr int WARP = D8_SLOTS * SLOT;
-    static constexpr int META = D8_NW * WARP;    // [warp][DEC_GP] float4, see Decode8State::store
-    static constexpr int WEIGHTS = META + D8_NW * DEC_GP * 16;  // the same: {of O, of the sum, largest score of the group, -}
-    static constexpr int bytes = WEIGHTS + D8_NW * DEC_GP * 16;
+    static constexpr int META = NW * WARP;    // [warp][DEC_GP] float4, see Decode8State::store
+    static constexpr int WEIGHTS = META + NW * DEC_GP * 16;  // the same: {of O, of the sum, largest score of the group, -}
+    static constexpr int bytes = WEIGHTS + NW * DEC_GP * 16;
     static_assert(SLOT >= DEC_GP * D * 4, "a warp's output fits the slot it has just used");
 };
 
@@ -204,8 +210,11 @@ __device__ __forceinline__ void d8_prefetch_q(const Decode8Params& P, int b, int
 }
 
 // Query heads first, first + step, .. of the group into `digits`, a warp; D = 64: two at a time.  Heads past the last: factor 0, and
-// whatever lies there as digits (whole numbers, so their scores are zeros).
-template <int D>
+// whatever lies there as digits (whole numbers, so their scores are zeros).  LOW: the three digits behind those, of what is left of an
+// element without them, times 2^23.  f32 arithmetic keeps 24 bits of every element however far apart they lie.  With 22 bits of the largest
+// alone, one element r times the others, where the keys are zero, puts the result off by 1.1e-6 for r = 30 and 3.6e-5 for r = 1000; with both
+// levels by nothing up to r = 2^21 and by 1.5e-9 for 10^6.
+template <int D, bool LOW = false>
 __device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk, int first, int step, uint32_t* digits, int lane) {
     constexpr int PER = 128 / D, ROW = Decode8Digits<D>::ROW;  // heads at a time
     const int word = lane % (D / 4), sub = lane / (D / 4);
@@ -244,12 +253,16 @@ __device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk,
                 }
             }
             const uint32_t big = __reduce_max_sync(mates, max(max(abs_bits(x[0]), abs_bits(x[1])), max(abs_bits(x[2]), abs_bits(x[3]))));
-            // 2^up q is at most 126 * 2^16 (up at most 100: the factor back stays a normal number)
+            // 2^up q is below 127 * 2^16 (up at most 100: the factor back stays a normal number)
             const int up = min(16 + 133 - (int)((big + 0x20000u) >> 23), 100);
             const float factor = __uint_as_float((uint32_t)(127 + up) << 23);
             uint32_t n[4];  // with 128 added to each digit they are the bytes; flipping the top bit takes it off again
 #pragma unroll
-            for (int e = 0; e < 4; ++e) n[e] = (uint32_t)(__float2int_rn(x[e] * factor) + 0x808080);
+            for (int e = 0; e < 4; ++e) {
+                const float y = x[e] * factor;
+                const int whole = __float2int_rn(y);  // (below 2^23: y - whole is exact, at most a half)
+                n[e] = (uint32_t)((LOW ? __float2int_rn((y - (float)whole) * 0x1p23f) : whole) + 0x808080);
+            }
             const uint32_t lo01 = __byte_perm(n[0], n[1], 0x5140), lo23 = __byte_perm(n[2], n[3], 0x5140);
             const uint32_t hi = __byte_perm(__byte_perm(n[0], n[1], 0x0062), __byte_perm(n[2], n[3], 0x0062), 0x5410);
             uint32_t* out = digits + h * ROW + word;
@@ -264,23 +277,29 @@ __device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk,
 }
 
 // A warp's state over one (sequence, kv head).  A lane holds columns (query heads) 2 (lane % 4) and the next.
-template <int D>
+template <int D, int LEVELS>
 struct Decode8State {
-    uint32_t q[3][D / 32][2];  // B fragments of Q^T, column lane / 4: the digits of the query, base 256, largest first
+    uint32_t q[3 * LEVELS][D / 32][2];  // B fragments of Q^T, column lane / 4: the digits of the query, base 256, largest first
     float qs[2];               // what turns a sum of digits times codes into a score in log2 units, but for the row's step
     float top[2];              // largest score so far
     float m[2], mv[2];         // references of the sum and of the output
     float l[2];
     float o[D / 16][4];        // [dims 16 c + 2 (lane / 4), next][columns]: (d, col), (d, col + 1), (d + 1, col), (d + 1, col + 1)
 
-    // The query from what d8_digits has left in shared memory, and the state before the first page.
-    __device__ __forceinline__ void start(const uint32_t* digits, int lane) {
+    // A level of digits from what d8_digits has left in shared memory.
+    __device__ __forceinline__ void load(const uint32_t* digits, int level, int lane) {
         constexpr int ROW = Decode8Digits<D>::ROW;
-        const int t = lane & 3;
 #pragma unroll
         for (int k = 0; k < 3; ++k)
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) q[k][c >> 1][c & 1] = digits[(k * DEC_GP + (lane >> 2)) * ROW + 4 * c + t];
+            for (int c = 0; c < D / 16; ++c) q[3 * level + k][c >> 1][c & 1] = digits[(k * DEC_GP + (lane >> 2)) * ROW + 4 * c + (lane & 3)];
+    }
+
+    // The first level with its factors, and the state before the first page.
+    __device__ __forceinline__ void start(const uint32_t* digits, int lane) {
+        constexpr int ROW = Decode8Digits<D>::ROW;
+        const int t = lane & 3;
+        load(digits, 0, lane);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             qs[j] = __uint_as_float(digits[3 * DEC_GP * ROW + 2 * t + j]);
@@ -292,6 +311,20 @@ struct Decode8State {
         for (int c = 0; c < D / 16; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.0f;
     }
 
+    // A level's digits times the codes, tokens gl and gl + 8 and this lane's columns: whole numbers, rounded to f32.
+    __device__ __forceinline__ void products(float (&x)[4], uint32_t frag, int level) const {
+        int acc[3][4] = {};
+#pragma unroll
+        for (int c = 0; c < D / 16; c += 2) {
+            uint32_t a[4];
+            ldmatrix_x4(a, frag ^ (c << 4));
+#pragma unroll
+            for (int k = 0; k < 3; ++k) mma_s8_16832(acc[k], a, q[3 * level + k][c >> 1][0], q[3 * level + k][c >> 1][1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fmaf((float)acc[0][e], 65536.0f, (float)(acc[1][e] * 256 + acc[2][e]));
+    }
+
     // One page in shared memory, tokens tok0 .. tok0 + 15 of which 0 .. len - 1 exist.  Whole warp.
     // frag: slot + d8_frag.
     __device__ __forceinline__ void page(uint32_t frag, uint32_t scale_slot, int tok0, int len, int lane) {
@@ -301,13 +334,13 @@ struct Decode8State {
         uint32_t byte;
         asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_slot + lane) : "memory");
         // ---- S^T = K Q^T: rows gl and gl + 8 (tokens), this lane's two columns
-        int acc[3][4] = {};
+        float x[4];
+        products(x, frag, 0);
+        if (LEVELS > 1) {  // (both in one loop, with six accumulators: 121 against 120 us, D = 64 77 against 74.5)
+            float y[4];
+            products(y, frag, LEVELS - 1);
 #pragma unroll
-        for (int c = 0; c < D / 16; c += 2) {
-            uint32_t a[4];
-            ldmatrix_x4(a, frag ^ (c << 4));
-#pragma unroll
-            for (int k = 0; k < 3; ++k) mma_s8_16832(acc[k], a, q[k][c >> 1][0], q[k][c >> 1][1]);
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], 0x1p-23f, x[e]);
         }
         const float scale = byte == kRowNaN ? __uint_as_float(0x7fc00000u) : lane < DEC_PT ? __uint_as_float(byte << 23) : (float)((int)byte - 127);
         float s[4], sv[4];
@@ -317,7 +350,7 @@ struct Decode8State {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int e = 2 * i + j;
-                s[e] = fmaf((float)acc[0][e], 65536.0f, (float)(acc[1][e] * 256 + acc[2][e])) * (step * qs[j]);
+                s[e] = x[e] * (step * qs[j]);
                 sv[e] = s[e] + ve;
             }
         }
@@ -412,7 +445,7 @@ struct Decode8State {
     __device__ __forceinline__ void store(uint8_t* smem, int warp, int lane) const {
         const int gl = lane >> 2, t = lane & 3;
         float* out = reinterpret_cast<float*>(smem + warp * Decode8Smem<D>::WARP);
-        float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D>::META) + warp * DEC_GP;
+        float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D, d8_warps<D, LEVELS>>::META) + warp * DEC_GP;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (gl == 0) meta[2 * t + j] = make_float4(m[j], l[j], mv[j] - D8_SHIFT, 0.0f);
@@ -492,7 +525,8 @@ struct Decode8Ring {
 #pragma unroll
         for (uint32_t at = 0; at < LAST; at += SLOT) d8_copy<D>(P, feed, place + at, base + at + 2 * DEC_PT * D, lane);
     }
-    __device__ __forceinline__ void page(const Decode8Params& P, Decode8Feed& feed, Decode8State<D>& st, int tok0, int len, int lane) {
+    template <int LEVELS>
+    __device__ __forceinline__ void page(const Decode8Params& P, Decode8Feed& feed, Decode8State<D, LEVELS>& st, int tok0, int len, int lane) {
         cp_async_wait<D8_SLOTS - 2>();
         __syncwarp();  // the page is there, and every lane is done with the slot before it
         d8_copy<D>(P, feed, place + spare, base + spare + 2 * DEC_PT * D, lane);
@@ -505,17 +539,17 @@ struct Decode8Ring {
 // The CTA's merge of its warps' states (Decode8State::store has put them at smem + w * WARP and to meta).  ends_with[w]: which warps belong
 // together, neighbours; < 0: none.  First every (warp, head) its weight next to its group's largest score, then the sums, where nothing
 // waits for anything.  done(w0, group size, rr, dg, M, L, acc) gets the group's first warp and the sums of dims 4 dg .. 4 dg + 3.
-template <int D, class Done>
+template <int D, int NW, class Done>
 __device__ __forceinline__ void d8_merge_warps(uint8_t* smem, const int* ends_with, int g, Done done) {
-    float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D>::META);
-    float4* weights = reinterpret_cast<float4*>(smem + Decode8Smem<D>::WEIGHTS);
+    float4* meta = reinterpret_cast<float4*>(smem + Decode8Smem<D, NW>::META);
+    float4* weights = reinterpret_cast<float4*>(smem + Decode8Smem<D, NW>::WEIGHTS);
     const int tid = threadIdx.x, lane = tid & 31;
     __syncthreads();
-    const int pair = lane < D8_NW ? ends_with[lane] : -1, before = __shfl_up_sync(0xffffffffu, pair, 1);
+    const int pair = lane < NW ? ends_with[lane] : -1, before = __shfl_up_sync(0xffffffffu, pair, 1);
     const unsigned joins = __ballot_sync(0xffffffffu, lane > 0 && pair >= 0 && pair == before);  // warps that go with the one before
     const unsigned leads = __ballot_sync(0xffffffffu, pair >= 0) & ~joins;
     const auto size_of = [&](int w0) { return __ffs(~(joins >> (w0 + 1))); };
-    if (tid < D8_NW * DEC_GP) {
+    if (tid < NW * DEC_GP) {
         const int w = tid / DEC_GP, rr = tid % DEC_GP;
         const unsigned upto = leads & ((2u << w) - 1);  // the last of them is this warp's group's, if it has one
         const int w0 = 31 - __clz(upto | 1);
@@ -529,7 +563,7 @@ __device__ __forceinline__ void d8_merge_warps(uint8_t* smem, const int* ends_wi
     }
     __syncthreads();
     const int items = __popc(leads) * g * (D / 4);
-    for (int item = tid; item < items; item += D8_THREADS) {
+    for (int item = tid; item < items; item += NW * 32) {
         const int dg = item % (D / 4), row = item / (D / 4), rr = row % g;
         unsigned from = leads;
         for (int k = row / g; k > 0; --k) from &= from - 1;
@@ -555,6 +589,7 @@ __device__ __forceinline__ void d8_merge_warps(uint8_t* smem, const int* ends_wi
 
 // The records of a (sequence, kv head) whose pages are [page0, page0 + np) of T, when more than one share has pages of it: one for each
 // CTA in which it is what shares end with, in the slot of the first of them, and one of the share that it ends inside of, if any.
+template <int NW>
 struct Decode8Records {
     int c_first, c_last;  // its shares
     int cta, groups, n;   // CTA of the first share; CTAs with a record of their shares; records
@@ -563,17 +598,17 @@ struct Decode8Records {
         c_first = deal.owner(page0);
         c_last = deal.owner(page0 + np - 1);
         const int inside = deal.bound(c_last + 1) > page0 + np;
-        cta = c_first / D8_NW;
-        groups = (c_last - inside) / D8_NW - cta + 1;
+        cta = c_first / NW;
+        groups = (c_last - inside) / NW - cta + 1;
         n = groups + inside;
     }
-    __device__ __forceinline__ int share(int i) const { return i == 0 ? c_first : i < groups ? (cta + i) * D8_NW : c_last; }
+    __device__ __forceinline__ int share(int i) const { return i == 0 ? c_first : i < groups ? (cta + i) * NW : c_last; }
 };
 
 // One query head's records merged to its result, by a warp; other CTAs have written them, so nothing of them is read from L1.  The loads
 // of eight records do not wait for their weights.
-template <int D>
-__device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const Decode8Records& R, int pair, int rr, int lane) {
+template <int D, int NW>
+__device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const Decode8Records<NW>& R, int pair, int rr, int lane) {
     constexpr int E = D / 32, BATCH = 8;
     const int b = pair / P.Hkv, hk = pair % P.Hkv;
     float M = -INFINITY, L = 0.0f, acc[E] = {};
@@ -629,16 +664,17 @@ __device__ __forceinline__ void d8_merge_records(const Decode8Params& P, const D
 // its registers to the result.  What a warp ends with is merged with the warps of the CTA that end with the same pair, to one
 // record, or to the result when the CTA has all of it.  Of the pairs that it shares with other CTAs it adds the pages it had to a counter,
 // and merges the records of those that are complete with it: no second launch, and no order of arrival in a result.
-template <int D>
-__global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __grid_constant__ Decode8Params P, const int shares) {
-    using Smem = Decode8Smem<D>;
+template <int D, int LEVELS>
+__global__ void __launch_bounds__(d8_warps<D, LEVELS> * 32, 1) decode8_splitkv_kernel(const __grid_constant__ Decode8Params P, const int shares) {
+    constexpr int NW = d8_warps<D, LEVELS>;
+    using Smem = Decode8Smem<D, NW>;
     extern __shared__ __align__(128) uint8_t d8_smem[];
-    __shared__ int ends_with[D8_NW];  // the pair that a warp's last pages belong to, -1 when there is nothing to merge
-    __shared__ int4 parts[2 * D8_NW]; // what a warp begins and ends with, when it has not all of it: {pair, first page of it, pages here, pages}
-    __shared__ struct { int pair; Decode8Records records; } complete[2 * D8_NW];
+    __shared__ int ends_with[NW];     // the pair that a warp's last pages belong to, -1 when there is nothing to merge
+    __shared__ int4 parts[2 * NW];    // what a warp begins and ends with, when it has not all of it: {pair, first page of it, pages here, pages}
+    __shared__ struct { int pair; Decode8Records<NW> records; } complete[2 * NW];
     __shared__ int n_complete;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int cta0 = (int)blockIdx.x * D8_NW, share = cta0 + warp;
+    const int cta0 = (int)blockIdx.x * NW, share = cta0 + warp;
     after_previous_launch();
     // T pages in all
     int sum = 0;
@@ -681,7 +717,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     ring.fill(P, feed, lane);
 
     if (P.res.mode != 2)  // sequences without pages (mode 0: in a replay only): empty records, zeros
-        for (int row = (int)blockIdx.x * D8_THREADS + tid; row < P.B * P.res.Hq; row += gridDim.x * D8_THREADS)
+        for (int row = (int)blockIdx.x * NW * 32 + tid; row < P.B * P.res.Hq; row += gridDim.x * NW * 32)
             if (P.end[row / P.res.Hq] == 0) {
                 const int b = row / P.res.Hq, h = row % P.res.Hq;
                 for (int dg = 0; dg < D / 4; ++dg)
@@ -689,7 +725,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
             }
     if (tid == 0) n_complete = 0;
     if (lane < 2) parts[2 * warp + lane] = make_int4(0, 0, 0, 0);
-    Decode8State<D> st;
+    Decode8State<D, LEVELS> st;
     int open = -1;
     for (int i = 0; i < n; w.next(P)) {
         const int seg_end = min(n, w.off + w.np);
@@ -699,6 +735,12 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
         d8_digits<D>(P, w.b, w.hk, 0, 1, digits, lane);
         __syncwarp();
         st.start(digits, lane);
+        if (LEVELS > 1) {
+            __syncwarp();
+            d8_digits<D, true>(P, w.b, w.hk, 0, 1, digits, lane);
+            __syncwarp();
+            st.load(digits, LEVELS - 1, lane);
+        }
         for (int tok0 = (i - w.off) * DEC_PT - front; i < seg_end; ++i, tok0 += DEC_PT) ring.page(P, feed, st, tok0, len, lane);
         st.reduce();
         const int pair = w.b * P.Hkv + w.hk;
@@ -715,13 +757,13 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
         if (i >= n) break;
     }
     if (lane == 0) ends_with[warp] = open;
-    const int cta_first = deal.bound(cta0), cta_end = deal.bound(cta0 + D8_NW);
+    const int cta_first = deal.bound(cta0), cta_end = deal.bound(cta0 + NW);
     const auto inside = [&](int4 part) { return part.y >= cta_first && part.y + part.w <= cta_end && P.res.mode != 2; };  // all its pages are this CTA's
-    d8_merge_warps<D>(d8_smem, ends_with, P.g, [&](int w0, int size, int rr, int dg, float M, float L, float4 acc) {
+    d8_merge_warps<D, NW>(d8_smem, ends_with, P.g, [&](int w0, int size, int rr, int dg, float M, float L, float4 acc) {
         const int pair = ends_with[w0];
         const long long rec = ((long long)pair + cta0 + w0) * DEC_GP + rr;
         if (inside(parts[2 * w0 + 1])) {
-            if (w0 + size < D8_NW && parts[2 * (w0 + size)].z > 0 && parts[2 * (w0 + size)].x == pair) {  // and the record of the warp that it ends inside of
+            if (w0 + size < NW && parts[2 * (w0 + size)].z > 0 && parts[2 * (w0 + size)].x == pair) {  // and the record of the warp that it ends inside of
                 const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + (rec + size * DEC_GP) * 2);
                 const float4 o = *reinterpret_cast<const float4*>(P.part_o + (rec + size * DEC_GP) * D + dg * 4);
                 const float top = fmaxf(M, ml.x), a0 = L == 0.0f ? 0.0f : fast_exp2(M - top), a1 = ml.y == 0.0f ? 0.0f : fast_exp2(ml.x - top);
@@ -744,10 +786,10 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     // ---- the pairs that are complete with this CTA's pages
     __threadfence();
     __syncthreads();  // this CTA's records can be seen everywhere
-    if (tid < 2 * D8_NW && parts[tid].z > 0 && !inside(parts[tid])) {
+    if (tid < 2 * NW && parts[tid].z > 0 && !inside(parts[tid])) {
         const int4 part = parts[tid];
         const int pair = part.x, before = atomicAdd(P.done + pair, part.z);
-        const Decode8Records R(deal, part.y, part.w);
+        const Decode8Records<NW> R(deal, part.y, part.w);
         if (before + part.z == part.w) {
             P.done[pair] = 0;
             complete[atomicAdd(&n_complete, 1)] = {pair, R};
@@ -755,28 +797,28 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_splitkv_kernel(const __
     }
     __threadfence();
     __syncthreads();
-    for (int item = warp; item < n_complete * P.g; item += D8_NW)
-        d8_merge_records<D>(P, complete[item / P.g].records, complete[item / P.g].pair, item % P.g, lane);
+    for (int item = warp; item < n_complete * P.g; item += NW)
+        d8_merge_records<D, NW>(P, complete[item / P.g].records, complete[item / P.g].pair, item % P.g, lane);
 }
 
 // Few pages: a cluster of C CTAs per (sequence, kv head), as decode_cluster_kernel: one launch, the CTAs' states meet in shared
 // memory over the cluster.  Bound by latencies: of 6.6 us for 1411 tokens (H32/8 D128, medians of time stamps, without the overlap with the launch before) 1.4 go to the
 // lengths, 0.5 to the page table, 0.6 to the query's digits, 1.4 to the pages, 1.4 to the CTA's merge, 1.2 to the cluster's.  Back to back in
 // graphs 7.5 to 7.6, where the bf16 cache takes 6.4: so few pages gain nothing from being half as long.
-template <int D>
+template <int D, int NW>
 struct Decode8ClusterSmem {
     static constexpr int SLOT_F4 = DEC_GP * D / 4 + DCL_MAX;  // column groups pushed here by all CTAs (rounded up per source)
-    static constexpr int PUSH = Decode8Smem<D>::bytes;
+    static constexpr int PUSH = Decode8Smem<D, NW>::bytes;
     static constexpr int bytes = PUSH + SLOT_F4 * 16 + DCL_MAX * DEC_GP * 8;
 };
 
-template <int D>
-__global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __grid_constant__ Decode8Params P, const int C) {
-    constexpr int DG = D / 4;
+template <int D, int LEVELS>
+__global__ void __launch_bounds__(d8_warps<D, LEVELS> * 32, 1) decode8_cluster_kernel(const __grid_constant__ Decode8Params P, const int C) {
+    constexpr int DG = D / 4, NW = d8_warps<D, LEVELS>;
     extern __shared__ __align__(128) uint8_t d8_smem[];
-    __shared__ int ends_with[D8_NW];
-    float4* push = reinterpret_cast<float4*>(d8_smem + Decode8ClusterSmem<D>::PUSH);       // [source CTA][column group of this CTA]
-    float2* push_ml = reinterpret_cast<float2*>(push + Decode8ClusterSmem<D>::SLOT_F4);    // [source CTA][GP]
+    __shared__ int ends_with[NW];
+    float4* push = reinterpret_cast<float4*>(d8_smem + Decode8ClusterSmem<D, NW>::PUSH);       // [source CTA][column group of this CTA]
+    float2* push_ml = reinterpret_cast<float2*>(push + Decode8ClusterSmem<D, NW>::SLOT_F4);    // [source CTA][GP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = C > 1 ? (int)cluster_cta_rank() : 0;
     after_previous_launch();
@@ -788,15 +830,19 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
     Decode8Ring<D> ring(d8_smem, warp, lane);
     const Decode8Walk start{b, hk, pages, -p_begin};
     Decode8Feed feed;
-    feed.init(P, start, warp, n, D8_NW);
+    feed.init(P, start, warp, n, NW);
     ring.fill(P, feed, lane);
-    uint32_t* digits = reinterpret_cast<uint32_t*>(d8_smem + ring.spare);  // warp 0's
-    if (warp < DEC_GP * D / 128) d8_digits<D>(P, b, hk, warp, DEC_GP * D / 128, digits, lane);
+    uint32_t* digits = reinterpret_cast<uint32_t*>(d8_smem + ring.spare);  // warp 0's, of the second level warp 1's
+    uint32_t* low_digits = reinterpret_cast<uint32_t*>(d8_smem + Decode8Smem<D>::WARP + ring.spare);
+    constexpr int MAKERS = DEC_GP * D / 128 * LEVELS > NW ? NW / LEVELS : DEC_GP * D / 128;  // warps that make a level
+    if (warp < MAKERS) d8_digits<D>(P, b, hk, warp, MAKERS, digits, lane);
+    else if (LEVELS > 1 && warp < 2 * MAKERS) d8_digits<D, true>(P, b, hk, warp - MAKERS, MAKERS, low_digits, lane);
     __syncthreads();
-    Decode8State<D> st;
+    Decode8State<D, LEVELS> st;
     st.start(digits, lane);
+    if (LEVELS > 1) st.load(low_digits, LEVELS - 1, lane);
     __syncthreads();
-    for (int i = warp; i < n; i += D8_NW) ring.page(P, feed, st, (p_begin + i) * DEC_PT - front, end - front, lane);
+    for (int i = warp; i < n; i += NW) ring.page(P, feed, st, (p_begin + i) * DEC_PT - front, end - front, lane);
     cp_async_wait<0>();
     __syncwarp();  // nothing is on its way to the slots any more
     st.reduce();
@@ -804,7 +850,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
     if (lane == 0) ends_with[warp] = 0;
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster has started
     const int items = P.g * DG, per = (items + C - 1) / C;  // CTA k finishes column groups [k per, (k + 1) per)
-    d8_merge_warps<D>(d8_smem, ends_with, P.g, [&](int, int, int rr, int dg, float M, float L, float4 acc) {
+    d8_merge_warps<D, NW>(d8_smem, ends_with, P.g, [&](int, int, int rr, int dg, float M, float L, float4 acc) {
         if (C == 1) {
             decode_emit(P.res, D, P.g, b, hk, rr, dg, M, L, acc);
         } else {
@@ -816,7 +862,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
     if (C == 1) return;
     __syncwarp();
     cluster_sync();  // everything pushed here has arrived
-    for (int item = rank * per + tid; item < min(items, (rank + 1) * per); item += D8_THREADS) {
+    for (int item = rank * per + tid; item < min(items, (rank + 1) * per); item += NW * 32) {
         const int rr = item / DG, dg = item % DG;
         float M = -INFINITY, L = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -831,6 +877,22 @@ __global__ void __launch_bounds__(D8_THREADS, 1) decode8_cluster_kernel(const __
         }
         decode_emit(P.res, D, P.g, b, hk, rr, dg, M, L, acc);
     }
+}
+
+// The two kernels of a head_dim and a type of query, as the host launches them
+struct Decode8Kernels {
+    void (*deal)(Decode8Params, int);
+    void (*cluster)(Decode8Params, int);
+    int warps, deal_smem, cluster_smem;
+};
+template <int D, int LEVELS>
+Decode8Kernels decode8_kernels_of() {
+    constexpr int NW = d8_warps<D, LEVELS>;
+    return {decode8_splitkv_kernel<D, LEVELS>, decode8_cluster_kernel<D, LEVELS>, NW, Decode8Smem<D, NW>::bytes, Decode8ClusterSmem<D, NW>::bytes};
+}
+inline Decode8Kernels decode8_kernels(int D, bool f32) {
+    if (D == 128) return f32 ? decode8_kernels_of<128, 2>() : decode8_kernels_of<128, 1>();
+    return f32 ? decode8_kernels_of<64, 2>() : decode8_kernels_of<64, 1>();
 }
 
 }  // namespace fusor

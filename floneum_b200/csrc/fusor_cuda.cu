@@ -363,6 +363,7 @@ extern "C" int32_t fusor_cuda_ctx_create(int32_t device, void* stream, fusor_cud
     ctx->pool.init(prop.totalGlobalMem / 64, reinterpret_cast<BufferPool::AddressRange>(range));
     // opt in to large dynamic shared memory once per context (each call is checked by its own return value: a kernel
     // whose static shared memory pushes the sum over the limit must fail here, not at its first launch)
+    const Decode8Kernels d8[4] = {decode8_kernels(128, false), decode8_kernels(64, false), decode8_kernels(128, true), decode8_kernels(64, true)};
     struct { const void* fn; int bytes; const char* name; } opt_in[] = {
         {(const void*)prefill_sm100_kernel<false, 0>, (int)PF_SMEM_BYTES, "prefill_sm100_kernel"},
         {(const void*)prefill_sm100_kernel<false, 1>, (int)PF_SMEM_BYTES, "prefill_sm100_kernel"},
@@ -379,10 +380,14 @@ extern "C" int32_t fusor_cuda_ctx_create(int32_t device, void* stream, fusor_cud
         {(const void*)decode_splitkv_kernel<64>, 227 * 1024, "decode_splitkv_kernel<64>"},
         {(const void*)decode_cluster_kernel<128>, (int)DecodeClusterSmem<128>::bytes, "decode_cluster_kernel<128>"},
         {(const void*)decode_cluster_kernel<64>, (int)DecodeClusterSmem<64>::bytes, "decode_cluster_kernel<64>"},
-        {(const void*)decode8_splitkv_kernel<128>, Decode8Smem<128>::bytes, "decode8_splitkv_kernel<128>"},
-        {(const void*)decode8_splitkv_kernel<64>, Decode8Smem<64>::bytes, "decode8_splitkv_kernel<64>"},
-        {(const void*)decode8_cluster_kernel<128>, Decode8ClusterSmem<128>::bytes, "decode8_cluster_kernel<128>"},
-        {(const void*)decode8_cluster_kernel<64>, Decode8ClusterSmem<64>::bytes, "decode8_cluster_kernel<64>"},
+        {(const void*)d8[0].deal, d8[0].deal_smem, "decode8_splitkv_kernel<128, 1>"},
+        {(const void*)d8[1].deal, d8[1].deal_smem, "decode8_splitkv_kernel<64, 1>"},
+        {(const void*)d8[2].deal, d8[2].deal_smem, "decode8_splitkv_kernel<128, 2>"},
+        {(const void*)d8[3].deal, d8[3].deal_smem, "decode8_splitkv_kernel<64, 2>"},
+        {(const void*)d8[0].cluster, d8[0].cluster_smem, "decode8_cluster_kernel<128, 1>"},
+        {(const void*)d8[1].cluster, d8[1].cluster_smem, "decode8_cluster_kernel<64, 1>"},
+        {(const void*)d8[2].cluster, d8[2].cluster_smem, "decode8_cluster_kernel<128, 2>"},
+        {(const void*)d8[3].cluster, d8[3].cluster_smem, "decode8_cluster_kernel<64, 2>"},
         {(const void*)attn_mma16_kernel<96, false, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, false, true>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
         {(const void*)attn_mma16_kernel<96, true, false>, (int)am_smem_bytes<96>, "attn_mma16_kernel<96>"},
@@ -1947,6 +1952,7 @@ static int32_t launch_combine(fusor_cuda_kvcache* c, const DecodeOutput& res, in
 // Decode over 8-bit pages, `total` (page, kv head) pairs in all: see decode8.cuh.
 static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, long long total, fusor_cuda_exchange* ex) {
     fusor_cuda_ctx* ctx = c->ctx;
+    const Decode8Kernels K = decode8_kernels(c->D, P.q_dtype == FUSOR_CUDA_F32);
     long long longest = 0;
     for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
     const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;  // bytes of a page pair
@@ -1964,15 +1970,13 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
         const int C = 1 << i;
         const long long share = (longest + C - 1) / C;
         if (7200 + 93 * share * unit / 4096 <= 13000 + 98 * total / grid * unit / 4096) {
-            CUDA_TRY(ctx, launch_behind(ctx, c->D == 128 ? decode8_cluster_kernel<128> : decode8_cluster_kernel<64>, dim3((unsigned)(heads * C)), D8_THREADS,
-                                        c->D == 128 ? Decode8ClusterSmem<128>::bytes : Decode8ClusterSmem<64>::bytes, (unsigned)C, P, C));
+            CUDA_TRY(ctx, launch_behind(ctx, K.cluster, dim3((unsigned)(heads * C)), K.warps * 32, K.cluster_smem, (unsigned)C, P, C));
             return launch_check(ctx, "decode8_cluster_kernel");
         }
     }
-    const int shares = (int)std::min<long long>((long long)grid * D8_NW, total);  // every warp its share, at least a page of it
+    const int shares = (int)std::min<long long>((long long)grid * K.warps, total);  // every warp its share, at least a page of it
     if (total > 0) {  // (every chunk empty: only the merge kernel runs and writes empty records)
-        CUDA_TRY(ctx, launch_behind(ctx, c->D == 128 ? decode8_splitkv_kernel<128> : decode8_splitkv_kernel<64>, dim3((unsigned)((shares + D8_NW - 1) / D8_NW)),
-                                    D8_THREADS, c->D == 128 ? Decode8Smem<128>::bytes : Decode8Smem<64>::bytes, 1, P, shares));
+        CUDA_TRY(ctx, launch_behind(ctx, K.deal, dim3((unsigned)((shares + K.warps - 1) / K.warps)), K.warps * 32, K.deal_smem, 1, P, shares));
         TRY(launch_check(ctx, "decode8_splitkv_kernel"));
         if (P.res.mode != 2) return FUSOR_CUDA_OK;  // it merges its records itself
     }

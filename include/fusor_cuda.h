@@ -281,8 +281,9 @@ int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* cache, const fusor_cuda_te
 /* ------------------------------------------------------------------------------------------------
  * Decode: one query token per sequence against the paged cache (the Sq == 1 regime of the call site,
  * models/kalosm-llama/src/raw/attention_layer.rs:405-448; all-zero mask [1, kv_len]).
- *   q [B,Hq,1,D] (bf16, f16 or f32; rounded to bf16, the type of the cached keys; an 8-bit cache takes f32 queries to 22 bits of the
- *   head's largest element), out [B,Hq,1,D] (f32, bf16 or f16; rows start on a multiple of four elements).
+ *   q [B,Hq,1,D] (bf16, f16 or f32; rounded to bf16, the type of the cached keys; an 8-bit cache takes f32 queries to 45 bits of the
+ *   head's largest element, 16-bit ones to 22, which is all of an element from 2^-14 (f16: 2^-11) of it on), out [B,Hq,1,D] (f32,
+ *   bf16 or f16; rows start on a multiple of four elements).
  * Up to as many (sequence, kv head) pairs as SMs, with a longest sequence from 8 pages to a few thousand tokens: one launch, a
  * cluster of CTAs per pair.  Else split-KV: the pages of all (sequence, kv head) pairs are dealt evenly to a persistent grid by the kernel itself, from
  * the lengths on the device (a step after an append plans and uploads nothing on the host); each CTA emits a partial
