@@ -175,6 +175,10 @@ class PagedKvCache:
         """truncate_front without moving the kept rows: up to 15 evicted rows stay, skipped, in the first page."""
         self._ck(self._L.fusor_cuda_kvcache_drop_front(self._h, b, keep))
 
+    def set_window(self, tokens: int):
+        """Appends leave a sequence at most `tokens` rows: the oldest are dropped first, by calls that are not refused.  0: no window."""
+        self._ck(self._L.fusor_cuda_kvcache_set_window(self._h, tokens))
+
     def seq_len(self, b: int = 0) -> int:
         n = ctypes.c_int32()
         self._ck(self._L.fusor_cuda_kvcache_seq_len(self._h, b, ctypes.byref(n)))
@@ -346,31 +350,30 @@ class KvCache:
     def v(self) -> Optional[CachedKv]:
         return CachedKv(self, "v") if self.current_seq_len() else None
 
-    def _make_room(self, device: Device, k: Tensor, v: Tensor):
-        """Allocation on first use and the eviction rule of TensorCache::append; returns (k, v, rows dropped from the
-        front of the new tensors)."""
+    def _fit(self, device: Device, k: Tensor, v: Tensor):
+        """The paged cache for these rows, which drops the oldest as TensorCache::append does, the rows that survive, and how many
+        of the first do not.  Nothing of the cache changes before the append itself."""
         B, Hkv, n, D = k.shape()
         assert tuple(v.shape()) == (B, Hkv, n, D), "k and v shapes differ"
-        if self._paged is None or B > self._paged.max_batch or (self._num_kv_heads, self._head_dim) != (Hkv, D):
-            pages_per_seq = (self.max_sequence_len + PAGE_TOKENS - 1) // PAGE_TOKENS + 1
-            self._paged = PagedKvCache(device, B, Hkv, D, B * pages_per_seq, pages_per_seq, dtype=self.dtype)
-            self._num_kv_heads, self._head_dim = Hkv, D
-        mx = self.max_sequence_len
-        skip = 0
-        if n >= mx:  # only the newest max_sequence_len rows survive
-            self._paged.reset()
-            skip = n - mx
-            k = Tensor(device, k.ptr + skip * k.strides[2] * (4 if k.dtype == F32 else 2), (B, Hkv, mx, D), k.dtype, k.strides, owner=k)
-            v = Tensor(device, v.ptr + skip * v.strides[2] * (4 if v.dtype == F32 else 2), (B, Hkv, mx, D), v.dtype, v.strides, owner=v)
-        elif self.current_seq_len() + n > mx:
-            for b in range(B):
-                self._paged.drop_front(b, mx - n)
-        return k, v, skip
+        paged, mx = self._paged, self.max_sequence_len
+        if paged is None or B > paged.max_batch or (self._num_kv_heads, self._head_dim) != (Hkv, D):
+            pages_per_seq = (mx + PAGE_TOKENS - 1) // PAGE_TOKENS + 1
+            paged = PagedKvCache(device, B, Hkv, D, B * pages_per_seq, pages_per_seq, dtype=self.dtype)
+            paged.set_window(mx)
+        skip = max(0, n - mx)  # only the newest max_sequence_len rows survive
+        if skip:
+            k, v = (Tensor(device, t.ptr + skip * t.strides[2] * (4 if t.dtype == F32 else 2), (B, Hkv, mx, D), t.dtype, t.strides, owner=t) for t in (k, v))
+        return paged, k, v, skip
+
+    def _hold(self, paged: PagedKvCache, k: Tensor):
+        """`paged` is the cache now: rows of k's shape have been appended to it."""
+        self._paged = paged
+        self._batch, self._num_kv_heads, _, self._head_dim = k.shape()
 
     def append(self, device: Device, k: Tensor, v: Tensor) -> Tuple[CachedKv, CachedKv]:
-        k, v, _ = self._make_room(device, k, v)
-        self._paged.append(k, v)
-        self._batch = k.shape()[0]
+        paged, k, v, _ = self._fit(device, k, v)
+        paged.append(k, v)
+        self._hold(paged, k)
         return CachedKv(self, "k"), CachedKv(self, "v")
 
     def _append_rotated(self, rope_cache, q: Tensor, k: Tensor, v: Tensor, start_pos: int, interleaved: bool, out_dtype,
@@ -378,16 +381,12 @@ class KvCache:
         """`RopeCache.forward(q, k, start_pos)` then `append(k, v)` in one launch (see RopeCache.forward_append)."""
         if start_pos < 0:
             start_pos = self.current_seq_len()
-        n = k.shape()[2]
-        if positions is not None or axes is not None:  # before any row gives way
-            from .rope import _positions
-            assert positions is not None and axes is not None, "positions and axes come together"
-            assert q.shape()[0] == k.shape()[0] and q.shape()[2:] == k.shape()[2:], f"q {list(q.shape())} and k {list(k.shape())} differ in batch, tokens or head_dim"
-            if self.current_seq_len() + n > self.max_sequence_len:
-                _positions(positions, axes, k.shape()[0], n, k.shape()[3])
-        k2, v2, skip = self._make_room(q.device, k, v)
+        assert (positions is None) == (axes is None), "positions and axes come together"
+        paged, k2, v2, skip = self._fit(q.device, k, v)
         if skip:  # the rows that do not survive still rotate q; do that with the plain op and append the rest
             from .rope import rope, rope_axes
+            n, ps = k.shape()[2], q.shape()
+            assert ps[0] == k.shape()[0] and ps[2:] == k.shape()[2:], f"q {list(ps)} and k {list(k.shape())} differ in batch, tokens or head_dim"
             if positions is not None:
                 q_rot = rope_axes(q, rope_cache.cos, rope_cache.sin, positions, axes, interleaved, out_dtype)
                 ps = positions.shape()
@@ -397,10 +396,10 @@ class KvCache:
                 q_rot = rope(q, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype)
             dummy = Tensor(q.device, q.ptr + skip * q.strides[2] * (4 if q.dtype == F32 else 2),
                            (q.shape()[0], q.shape()[1], n - skip, q.shape()[3]), q.dtype, q.strides, owner=q)
-            self._paged.rope_append(dummy, k2, v2, rope_cache.cos, rope_cache.sin, start_pos + skip, interleaved, out_dtype, positions, axes)
+            paged.rope_append(dummy, k2, v2, rope_cache.cos, rope_cache.sin, start_pos + skip, interleaved, out_dtype, positions, axes)
         else:
-            q_rot = self._paged.rope_append(q, k2, v2, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype, positions, axes)
-        self._batch = k.shape()[0]
+            q_rot = paged.rope_append(q, k2, v2, rope_cache.cos, rope_cache.sin, start_pos, interleaved, out_dtype, positions, axes)
+        self._hold(paged, k)
         return q_rot, CachedKv(self, "k"), CachedKv(self, "v")
 
     # ------------------------------------------------------------------ session export / import

@@ -1149,6 +1149,7 @@ struct fusor_cuda_kvcache {
     // split-KV decode: the kernel deals the pages out itself from d_end, the host only sizes the grid
     int max_grid = 0, max_slots = 0;
     int decode_ctas = 0;              // 0 = automatic grid size
+    int window = 0;                   // rows an append leaves a sequence at most, 0 = as many as there are pages for
     float* part_o = nullptr;          // [max_slots][DEC_GP][D]
     float* part_ml = nullptr;         // [max_slots][DEC_GP][2]
     int* done = nullptr;              // 8-bit pages: [max_batch * Hkv], see Decode8Params
@@ -1299,6 +1300,8 @@ static int32_t kv_upload_tables(fusor_cuda_kvcache* c, const int* before, int B)
     c->table_dirty = c->lens_dirty = false;
     return FUSOR_CUDA_OK;
 }
+// Rows that an append of n tokens takes off the front of sequence b.
+static int kv_dropped(const fusor_cuda_kvcache* c, int b, int n) { return c->window > 0 ? std::min(c->h_kv_len[b], std::max(0, c->h_kv_len[b] + n - c->window)) : 0; }
 static int32_t kv_sync_tables(fusor_cuda_kvcache* c) { return kv_upload_tables(c, nullptr, 0); }
 static int32_t kv_keep_rows(fusor_cuda_kvcache* c, int b, int keep);
 
@@ -1317,17 +1320,27 @@ static int32_t kv_reserve(fusor_cuda_kvcache* c, const fusor_cuda_tensor4* k_new
                     c->Hkv, c->D);
     if (B <= 0 || B > c->max_batch || n <= 0) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "batch %d (max %d) or token count %d invalid", B, c->max_batch, n);
     if (k_new->stride[3] != 1 || v_new->stride[3] != 1) return fail(ctx, FUSOR_CUDA_UNSUPPORTED, "the head_dim axis must be contiguous");
-    if (c->active_B != 0 && c->active_B != B)
+    if (c->window > 0 && n > c->window) return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "%d tokens do not fit a window of %d", n, c->window);
+    const bool anew = n == c->window;  // no row of what is there stays
+    if (!anew && c->active_B != 0 && c->active_B != B)
         return fail(ctx, FUSOR_CUDA_SHAPE_MISMATCH, "cache holds %d sequences, append brings %d", c->active_B, B);
     DeviceGuard g(ctx->device);
-    int need = 0, least = 0;  // pages to map as the rows lie, and with no evicted rows among them
+    int need = 0, least = 0;  // pages to map as the rows will lie once the window has dropped its oldest, and with no evicted rows among them
+    int free_pages = anew ? c->num_pages : (int)c->free_list.size();
+    const auto dropped = [&](int b) { return kv_dropped(c, b, n); };
     for (int b = 0; b < B; ++b) {
-        const int want = pages_of(c->h_kv_len[b] + n);
+        const int drop = anew ? 0 : dropped(b), front = anew ? 0 : c->h_front[b] + drop, len = anew ? 0 : c->h_kv_len[b] - drop;
+        const int want = pages_of(len + n), end = front % DEC_PT + len;
         if (want > c->max_pages) return fail(ctx, FUSOR_CUDA_OUT_OF_PAGES, "sequence %d would need %d pages (max %d per sequence)", b, want, c->max_pages);
-        least += want - pages_of(kv_end(c, b));
-        need += pages_of(kv_end(c, b) + n) - pages_of(kv_end(c, b));
+        least += want - pages_of(end);
+        need += pages_of(end + n) - pages_of(end);
+        free_pages += front / DEC_PT;
     }
-    if (least > (int)c->free_list.size()) return fail(ctx, FUSOR_CUDA_OUT_OF_PAGES, "need %d pages, %d free", least, (int)c->free_list.size());
+    if (least > free_pages) return fail(ctx, FUSOR_CUDA_OUT_OF_PAGES, "need %d pages, %d free", least, free_pages);
+    // ---- nothing is refused from here on: the oldest rows give way
+    if (anew) TRY(fusor_cuda_kvcache_reset(c));
+    for (int b = 0; b < B; ++b)
+        if (dropped(b) > 0) TRY(fusor_cuda_kvcache_drop_front(c, b, c->window - n));
     // Evicted rows at a sequence's front must not cost it a page it may not have: its rows then move to the page's start.
     const bool tight = need > (int)c->free_list.size();
     need = 0;
@@ -1600,7 +1613,7 @@ extern "C" int32_t fusor_cuda_kvcache_rope_append(fusor_cuda_kvcache* c, const f
     long long last = (long long)start_pos + n;
     if (start_pos < 0) {
         last = 0;
-        for (int b = 0; b < B && b < c->max_batch; ++b) last = std::max<long long>(last, (long long)c->h_kv_len[b] + n);
+        for (int b = 0; b < B && b < c->max_batch; ++b) last = std::max<long long>(last, (long long)c->h_kv_len[b] - kv_dropped(c, b, n) + n);
     }
     if (last > context_length)
         return fail(ctx, FUSOR_CUDA_INVALID_ARGUMENT, "positions up to %lld are outside the %d-row cos/sin tables", last, context_length);
@@ -1636,6 +1649,13 @@ extern "C" int32_t fusor_cuda_kvcache_rope_axes_append(fusor_cuda_kvcache* c, co
     place_q(P, q, q_out, cos_t, sin_t, context_length, interleaved);
     TRY(place_positions(ctx, P, positions, c->D));
     return place_append(c, k_new, v_new, P);
+}
+
+extern "C" int32_t fusor_cuda_kvcache_set_window(fusor_cuda_kvcache* c, int32_t tokens) {
+    if (!c) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "cache is null");
+    if (tokens < 0) return kv_fail(c, FUSOR_CUDA_INVALID_ARGUMENT, "a window must not be negative");
+    c->window = tokens;
+    return FUSOR_CUDA_OK;
 }
 
 extern "C" int32_t fusor_cuda_kvcache_seq_len(fusor_cuda_kvcache* c, int32_t b, int32_t* len) {

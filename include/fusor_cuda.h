@@ -255,6 +255,11 @@ int32_t fusor_cuda_kvcache_truncate_front(fusor_cuda_kvcache* cache, int32_t b, 
  * rows move only when an append would otherwise need a page that the sequence or the pool does not have, or at the next
  * fusor_cuda_kvcache_truncate_front, whatever its `keep`. */
 int32_t fusor_cuda_kvcache_drop_front(fusor_cuda_kvcache* cache, int32_t b, int32_t keep);
+/* The same eviction as a part of every append, of any kind: one that would leave a sequence more than `tokens` rows drops its oldest
+ * first, once nothing about the call can be refused any more, so that a refused append leaves the cache as it was.  An append of
+ * `tokens` rows takes the place of all that is there, whatever its batch; longer ones are INVALID_ARGUMENT.  A start_pos < 0 counts what is
+ * left.  0 (default): no window. */
+int32_t fusor_cuda_kvcache_set_window(fusor_cuda_kvcache* cache, int32_t tokens);
 /* KvCache::current_seq_len (kv_cache.rs:65-67) of sequence b. */
 int32_t fusor_cuda_kvcache_seq_len(fusor_cuda_kvcache* cache, int32_t b, int32_t* len);
 /* Installs a caller-built mapping (host arrays): page_table [B][max_pages_per_seq], kv_len [B]. Entries beyond

@@ -333,30 +333,32 @@ class KvCache {
     std::pair<CachedKv, CachedKv> append(const DevicePtr& dev, const Tensor<4>& k, const Tensor<4>& v) {
         const auto& s = k.shape();
         if (v.shape() != s) throw std::logic_error("k and v shapes differ");
+        // nothing of this cache changes before the append itself, which drops the oldest rows when nothing can be refused any more
+        std::unique_ptr<fusor_cuda_kvcache, int32_t (*)(fusor_cuda_kvcache*)> made(nullptr, fusor_cuda_kvcache_destroy);
         if (!cache_ || s[0] > max_batch_ || s[1] != hkv_ || s[3] != d_) {
-            if (cache_) fusor_cuda_kvcache_destroy(cache_);
-            cache_ = nullptr;
-            dev_ = dev;
             const int pages_per_seq = (int)((max_len_ + 15) / 16 + 1);
+            fusor_cuda_kvcache* c = nullptr;
             dev->check(fusor_cuda_kvcache_create_dtype(dev->raw(), (int32_t)s[0], (int32_t)s[1], (int32_t)s[3], 16, (int32_t)s[0] * pages_per_seq,
-                                                       pages_per_seq, cache_dtype_, &cache_));
+                                                       pages_per_seq, cache_dtype_, &c));
+            made.reset(c);
+            dev->check(fusor_cuda_kvcache_set_window(c, (int32_t)max_len_));
+        }
+        auto vk = detail::view4(k), vv = detail::view4(v);
+        if ((size_t)s[2] > max_len_) {  // only the newest max_sequence_len rows survive
+            const int64_t skip = s[2] - (int64_t)max_len_;
+            vk.data = (char*)vk.data + skip * vk.stride[2] * (k.dtype() == DType::F32 ? 4 : 2);
+            vv.data = (char*)vv.data + skip * vv.stride[2] * (v.dtype() == DType::F32 ? 4 : 2);
+            vk.shape[2] = vv.shape[2] = (int64_t)max_len_;
+        }
+        dev->check(fusor_cuda_kvcache_append(made ? made.get() : cache_, &vk, &vv));
+        if (made) {
+            if (cache_) fusor_cuda_kvcache_destroy(cache_);
+            cache_ = made.release();
+            dev_ = dev;
             max_batch_ = s[0];
             hkv_ = s[1];
             d_ = s[3];
         }
-        auto vk = detail::view4(k), vv = detail::view4(v);
-        const int64_t n = s[2];
-        if ((size_t)n >= max_len_) {  // only the newest max_sequence_len rows survive
-            dev_->check(fusor_cuda_kvcache_reset(cache_));
-            const int64_t skip = n - (int64_t)max_len_;
-            const size_t esz = k.dtype() == DType::F32 ? 4 : 2;
-            vk.data = (char*)vk.data + skip * vk.stride[2] * esz;
-            vv.data = (char*)vv.data + skip * vv.stride[2] * (v.dtype() == DType::F32 ? 4 : 2);
-            vk.shape[2] = vv.shape[2] = (int64_t)max_len_;
-        } else if (current_seq_len() + (size_t)n > max_len_) {
-            for (int64_t b = 0; b < s[0]; ++b) dev_->check(fusor_cuda_kvcache_drop_front(cache_, (int32_t)b, (int32_t)(max_len_ - n)));
-        }
-        dev_->check(fusor_cuda_kvcache_append(cache_, &vk, &vv));
         batch_ = s[0];
         return {CachedKv{this, true}, CachedKv{this, false}};
     }
