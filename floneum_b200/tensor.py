@@ -41,6 +41,15 @@ def _from_bf16_bits(b: np.ndarray) -> np.ndarray:
     return (b.astype(np.uint32) << 16).view(np.float32)
 
 
+def _whole_numbers(data) -> np.ndarray:
+    """Host data as u32; what u32 does not hold is refused."""
+    a = np.asarray(data)
+    if a.dtype != np.uint32 and a.size:
+        assert a.dtype.kind in "uifb" and a.min() >= 0 and a.max() < 2 ** 32 and (a.dtype.kind != "f" or not (a % 1).any()), (
+            "u32 data must be whole numbers from 0 to 2^32 - 1")
+    return a.astype(np.uint32)
+
+
 def _host_bits(a: np.ndarray, dtype: int) -> np.ndarray:
     """f32 host values -> the array that is uploaded for `dtype` (f16: numpy's own round-to-nearest-even)."""
     if dtype in (F32, U32):
@@ -82,7 +91,7 @@ class Tensor:
     @classmethod
     def from_slice(cls, device: Device, shape: Sequence[int], data, dtype: int = F32) -> "Tensor":
         """Upload host data (any array-like of floats, or of whole numbers for u32) as a contiguous tensor of `shape`."""
-        a = np.ascontiguousarray(np.asarray(data, dtype=np.uint32 if dtype == U32 else np.float32).reshape(shape))
+        a = np.ascontiguousarray((_whole_numbers(data) if dtype == U32 else np.asarray(data, dtype=np.float32)).reshape(shape))
         host = _host_bits(a, dtype)
         t = cls.empty(device, shape, dtype)
         L = _lib.load()
