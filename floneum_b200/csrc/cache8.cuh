@@ -70,7 +70,7 @@ struct PlaceParams {
 // Table row of pair i of token t of sequence b.  Rows outside the table are recorded and read as row 0.
 __device__ __forceinline__ int place_row(const PlaceParams& P, int b, int t, int i) {
     if (!P.pos) return (P.start_pos >= 0 ? P.start_pos : P.lens.before(b) - P.lens.evicted(b)) + t;
-    const uint32_t row = __ldg(P.pos + P.axis[i] * P.pos_axis + b * P.pos_b + t);
+    const uint32_t row = P.pos[P.axis[i] * P.pos_axis + b * P.pos_b + t];
     if (row < (uint32_t)P.context) return (int)row;
     atomicExch(P.err, kErrBadPosition);
     return 0;
@@ -106,6 +106,14 @@ __device__ __forceinline__ void place_floats(const uint4 (&raw)[PlaceType<T>::U4
     }
 }
 
+// Eight values of a table, by loads that stay behind after_previous_launch() (as do all of this kernel: the launch before may have written
+// positions and tables too).
+__device__ __forceinline__ void place_table8(const float* t, long long at, float (&f)[8]) {
+    const float4* v = reinterpret_cast<const float4*>(t + at);
+    const float4 a = v[0], b = v[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
 // cos and sin of pairs i0 .. i0 + 7 of token t of sequence b
 __device__ __forceinline__ void place_angles(const PlaceParams& P, int b, int t, int i0, float (&c)[8], float (&s)[8]) {
     const int half = P.D >> 1;
@@ -116,15 +124,15 @@ __device__ __forceinline__ void place_angles(const PlaceParams& P, int b, int t,
     }
     if (one) {
         const long long at = (long long)place_row(P, b, t, i0) * half + i0;
-        rope_load8(P.cos_t, 0, at, c);
-        rope_load8(P.sin_t, 0, at, s);
+        place_table8(P.cos_t, at, c);
+        place_table8(P.sin_t, at, s);
         return;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const long long at = (long long)place_row(P, b, t, i0 + j) * half + i0 + j;
-        c[j] = __ldg(P.cos_t + at);
-        s[j] = __ldg(P.sin_t + at);
+        c[j] = P.cos_t[at];
+        s[j] = P.sin_t[at];
     }
 }
 
