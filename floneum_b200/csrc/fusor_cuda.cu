@@ -1153,6 +1153,7 @@ struct fusor_cuda_kvcache {
     float* part_o = nullptr;          // [max_slots][DEC_GP][D]
     float* part_ml = nullptr;         // [max_slots][DEC_GP][2]
     int* done = nullptr;              // 8-bit pages: [max_batch * Hkv], see Decode8Params
+    bool done_stale = false;          // to be cleared before the next decode: the cache was reset
     // dense staging for token-granular eviction, grown on demand
     uint8_t* shift_buf = nullptr;
     size_t shift_bytes = 0;
@@ -1275,6 +1276,7 @@ extern "C" int32_t fusor_cuda_kvcache_reset(fusor_cuda_kvcache* c) {
     for (int i = 0; i < c->num_pages; ++i) c->free_list[i] = c->num_pages - 1 - i;
     c->active_B = 0;
     c->table_dirty = true;
+    c->done_stale = true;
     return FUSOR_CUDA_OK;
 }
 
@@ -1992,6 +1994,17 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
         if (7200 + 93 * share * unit / 4096 <= 13000 + 98 * total / grid * unit / 4096) {
             CUDA_TRY(ctx, launch_behind(ctx, K.cluster, dim3((unsigned)(heads * C)), K.warps * 32, K.cluster_smem, (unsigned)C, P, C));
             return launch_check(ctx, "decode8_cluster_kernel");
+        }
+    }
+    // Every decode leaves the counters at zero; two of one cache that ran at the same time may not have.  After a reset they are zero again.
+    // (Cleared here, not there: what follows a reset are appends, and a clear is an operation of its own.  Nor in a graph, whose every
+    // replay would have it.)
+    if (c->done_stale) {
+        cudaStreamCaptureStatus capture;
+        CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+        if (capture == cudaStreamCaptureStatusNone) {
+            CUDA_TRY(ctx, cudaMemsetAsync(c->done, 0, (size_t)c->max_batch * c->Hkv * 4, ctx->stream));
+            c->done_stale = false;
         }
     }
     const int shares = (int)std::min<long long>((long long)grid * K.warps, total);  // every warp its share, at least a page of it

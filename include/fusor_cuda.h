@@ -294,7 +294,8 @@ int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* cache, const fusor_cuda_te
  * the lengths on the device (a step after an append plans and uploads nothing on the host); each CTA emits a partial
  * (m, l, O) per run of pages, and a second kernel, which finds each head's partials with the same deal, merges them by
  * log-sum-exp (over 8-bit pages the CTA that completes a pair merges its partials: one launch).  Work of one cache shares its partials:
- * captured graphs that hold decodes of one cache must not run at the same time. */
+ * captured graphs that hold decodes of one cache must not run at the same time (over 8-bit pages the results are then right again only
+ * from the first call after a fusor_cuda_kvcache_reset on). */
 int32_t fusor_cuda_flash_attention_decode(fusor_cuda_ctx* ctx, fusor_cuda_kvcache* cache, const fusor_cuda_tensor4* q,
                                           float scale, const fusor_cuda_tensor4* out);
 /* Same, but leaves the result un-normalised for a merge across GPUs that each hold a chunk of the keys:

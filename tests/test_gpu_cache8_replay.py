@@ -69,3 +69,39 @@ def test_a_sequence_without_keys_gives_zeros(device, D, ctas, out):
             want, bound = attention(q[b, :, 0], *rows, scale)[0], attention_bound(q[b, :, 0], *rows, scale)
             assert (np.abs(got[b, 0] - want) <= bound + half * (np.abs(want) + bound)).all(), (now, b)
     del graph
+
+
+@pytest.mark.parametrize("window", [0, 900])
+def test_a_cache_that_was_reset(device, window):
+    """Decodes from many shares, eager and captured, between resets: each as from a cache of its own."""
+    import torch
+    fb = _fb()
+    stream = torch.cuda.Stream()
+    dev = fb.Device.gpu(0, stream.cuda_stream)
+    rng = np.random.default_rng(window)
+    D, scale = 64, 0.125
+    cache = fb.PagedKvCache(dev, 2, 2, D, 2 * 60, 60, dtype=fb.I8)
+    cache.set_window(window)
+    cache.set_decode_ctas(40)
+    for n in (900, 900, 33, 900):
+        k, v = (rng.standard_normal((2, 2, n, D)).astype(np.float32) for _ in range(2))
+        q = rng.standard_normal((2, 4, 1, D)).astype(np.float32)
+        if window == 0 or n < window:
+            cache.reset()
+        cache.append(_T(dev, k), _T(dev, v))
+        tq, out = _T(dev, q), fb.Tensor.zeros(dev, q.shape)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+            cache.decode(tq, scale, out=out)
+        got = []
+        for _ in range(2):
+            got.append(cache.decode(tq, scale).as_slice())
+            graph.replay()
+            torch.cuda.synchronize()
+            got.append(out.as_slice())
+        for g in got:
+            assert np.array_equal(g, got[0])
+            for b in range(2):
+                want, bound = attention(q[b, :, 0], held(k)[b], held(v)[b], scale)[0], attention_bound(q[b, :, 0], held(k)[b], held(v)[b], scale)
+                assert (np.abs(g[b, :, 0] - want) <= bound).all()
+        del graph
