@@ -10,8 +10,9 @@
 //    digits more for what is left, 45 bits together; of 16-bit ones an element below 2^-14 (f16: 2^-11) of its head's largest is off by up to
 //    2^-23 of that;
 //  * the weight of a value row is exp(s) 2^ve in one exponential, against a running reference of its own, so that rows whose steps
-//    lie far apart weigh in f16 as they do in the result: a factor of 2^6 and two terms, 22 bits down to 2^-31 of the reference.
-//    The value codes become f16 by setting the exponent of 1024 over the byte and subtracting: exact;
+//    lie far apart weigh in f16 as they do in the result: a factor of 2^6 and two terms, off by 2^-22 of the weight or, from 2^-9 of the
+//    reference on down, by 2^-31 of the reference.  The value codes become f16 by setting the exponent of 1024 over the byte and
+//    subtracting: exact;
 //  * the tensor core cuts f32 sums off towards zero: each page's products go to accumulators of their own, which are then added to the
 //    running output in f32.
 // The references (of the sum and of the output) follow the maxima lazily: a page whose scores exceed them by less than 2^8 leaves them.
