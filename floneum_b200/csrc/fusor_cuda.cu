@@ -1801,7 +1801,7 @@ extern "C" int32_t fusor_cuda_kvcache_gather(fusor_cuda_kvcache* c, const fusor_
     else
         run(kvcache_gather_page_kernel<1, 64, 0>, kvcache_gather_page_kernel<1, 64, 1>, kvcache_gather_page_kernel<1, 64, 2>, kvcache_gather_page_kernel<1, 64, 3>);
     CUDA_TRY(ctx, e);
-    return launch_check(ctx, "kvcache_gather_kernel");
+    return launch_check(ctx, "kvcache_gather_page_kernel");
 }
 
 // Takes `dp` whole pages off the front of a sequence's table row.
@@ -1979,7 +1979,7 @@ static int32_t decode8_launch(fusor_cuda_kvcache* c, const Decode8Params& P, lon
     for (int b = 0; b < P.B; ++b) longest = std::max<long long>(longest, pages_of(kv_end(c, b)));
     const long long heads = (long long)P.B * c->Hkv, unit = 2ll * DEC_PT * c->D;  // bytes of a page pair
     // CTAs of the even deal: a record per CTA and pair, which one CTA merges, so not more than 32 to a pair (one sequence of 64000
-    // tokens with one kv head: 38.7 us from 148 CTAs, 25.7 from 32)
+    // tokens with one kv head: 38.7 us from 148 CTAs, 25.7 from 32, behind a launch of its own kind 23.8; its bytes take 2.5)
     const int grid = c->decode_ctas > 0 ? c->decode_ctas : (int)std::min<long long>(ctx->num_sms, 32 * heads);
     // A cluster per (sequence, kv head), of the largest size of which all fit at once, while its longest share is short enough.  Measured
     // (ns, 4 KB page pairs): the cluster 7200 + 93 per page of that share, the deal 13000 + 98 per page of a CTA's.  One sequence of

@@ -67,6 +67,9 @@ def axes_of_sections(sections: Sequence[int], alternating: bool = False) -> np.n
     return out
 
 
+_BYTE = np.dtype(np.uint8)
+
+
 def _positions(positions: Tensor, axes, batch: int, n: int, head_dim: int):
     """The C view of positions (u32 [n_axes, n], the same for every sequence, or [n_axes, batch, n])."""
     assert positions.dtype == U32, "positions must be a u32 tensor"
@@ -76,13 +79,13 @@ def _positions(positions: Tensor, axes, batch: int, n: int, head_dim: int):
     assert n == 1 or strides[-1] == 1, "the token axis of the positions must be contiguous"
     given = np.asarray(axes)
     assert given.shape == (head_dim // 2,), f"axes must name the axis of each of {head_dim // 2} pairs, got {list(given.shape)}"
-    if given.dtype != np.uint8:  # (bytes travel as they are, and the call looks at them)
+    if given.dtype is not _BYTE:  # (bytes travel as they are, and the call looks at them)
         assert given.min() >= 0 and given.max() < min(shape[0], 256) and (given.dtype.kind in "uib" or not (given % 1).any()), (
             f"axes {given.tolist()} must be whole numbers from 0 to {shape[0] - 1}, the axes of the positions")
-    axis_of_pair = np.ascontiguousarray(given, dtype=np.uint8)
+        given = given.astype(np.uint8)
     p = _lib.RopePositions()
     p.ids, p.axis_stride, p.batch_stride = positions.ptr, strides[0], strides[1] if len(shape) == 3 else 0
-    p.n_axes, p.axis_of_pair = shape[0], axis_of_pair.tobytes()  # (the structure keeps the bytes)
+    p.n_axes, p.axis_of_pair = shape[0], given.tobytes()  # (the structure keeps the bytes)
     return p
 
 
