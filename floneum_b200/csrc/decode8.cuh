@@ -18,13 +18,12 @@
 // The references (of the sum and of the output) follow the maxima lazily: a page whose scores exceed them by less than 2^8 leaves them.
 // Error of an f32 result against 64 bits: 2.4e-7 to 3.5e-7 (2-norm), that of f32 arithmetic in torch 4.5e-7 to 1.1e-6.
 //
-// B64 kv 1024-8192 H32/8 D128, 610 MB: 110 to 112 us in graphs = 5.5 TB/s; the bf16 cache's kernels take 193 us for these sequences.  Time stamps (without the overlap with the
-// launch before):
-// dealt 1.5 us, first copies 4, first page used 6.5; pages done on average at 90, the last at 100; the last CTA ends at 108.  610 MB in
-// those 84 us are 7.2 TB/s: HBM is the bound in between, and the ends are latencies and the spread of the warps, which a deal at run
-// time would even out at the price of results that depend on it.  401 warp instructions a page with all ends (ALU 45 % busy, the tensor
-// pipe 32 %).  16-bit MMAs on converted keys took 519 a page and 130 us, 8-bit ones before each warp had a run of pages 135, with it and a
-// second launch for the merge 118.
+// B64 kv 1024-8192 H32/8 D128, 610 MB: 109 to 112 us in graphs = 5.5 TB/s, with f32 queries 119 to 121; the bf16 cache's kernels take 193 us for
+// these sequences.  Time stamps (without the overlap with the launch before): dealt 1.5 us, first copies 4, first page used 6.5; pages
+// done on average at 90, the last at 100; the last CTA ends at 108.  610 MB in those 84 us are 7.2 TB/s: HBM is the bound in between, and
+// the ends are latencies and the spread of the warps, which a deal at run time would even out at the price of results that depend on it.
+// 401 warp instructions a page with all ends (ALU 44 % busy, the tensor pipe 32 %).  16-bit MMAs on converted keys took 519 a page and
+// 130 us, 8-bit ones before each warp had a run of pages 135, with it and a second launch for the merge 118.
 #pragma once
 #include <cfloat>
 
