@@ -213,7 +213,7 @@ __device__ __forceinline__ void d8_prefetch_q(const Decode8Params& P, int b, int
 // whatever lies there as digits (whole numbers, so their scores are zeros).  LOW: the three digits behind those, of what is left of an
 // element without them, times 2^23.  f32 arithmetic keeps 24 bits of every element however far apart they lie.  With 22 bits of the largest
 // alone, one element r times the others, where the keys are zero, puts the result off by 1.1e-6 for r = 30 and 3.6e-5 for r = 1000; with both
-// levels by nothing up to r = 2^21 and by 1.5e-9 for 10^6.
+// levels by 6e-12 at most up to r = 30000 and by 1.5e-9 for 10^6.
 template <int D, bool LOW = false>
 __device__ __forceinline__ void d8_digits(const Decode8Params& P, int b, int hk, int first, int step, uint32_t* digits, int lane) {
     constexpr int PER = 128 / D, ROW = Decode8Digits<D>::ROW;  // heads at a time

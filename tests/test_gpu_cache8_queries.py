@@ -1,8 +1,9 @@
-"""8-bit decode of f32 queries whose elements lie far apart, and how near f32 results are to 64 bits."""
+"""8-bit decode of queries whose elements lie far apart, and how near f32 results are to 64 bits."""
 import numpy as np
 import pytest
 
-from cache8_oracle import attention, held
+from cache8_oracle import attention, attention_bound, held
+from oracle import oracle as O
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,29 @@ def test_f32_results_of_ordinary_queries(device, D, lens):
     k, v = (rng.standard_normal((1, 2, lens, D)).astype(np.float32) for _ in range(2))
     for off in _off(device, q, k, v, float(D ** -0.5), (0, 1, 40)):
         assert off <= NORM
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("r", [1, 100, 8000, 60000])
+def test_16_bit_queries_of_any_spread(device, D, dtype, r):
+    """Elements from 2^-14 (f16: 2^-11) of the largest on are exact, the others off by up to 2^-23 of it: what that makes of a score, and twice
+    that of a result, on top of the bound of exact queries."""
+    fb = _fb()
+    rng = np.random.default_rng(D + dtype)
+    q = rng.standard_normal((1, 4, 1, D)).astype(np.float32)
+    k, v = (rng.standard_normal((1, 1, 700, D)).astype(np.float32) for _ in range(2))
+    q[..., 5], k[..., 5] = r, 0.0
+    q = O.bf16_round(q) if dtype == 1 else q.astype(np.float16).astype(np.float32)
+    wk, wv, scale = held(k)[0], held(v)[0], float(D ** -0.5)
+    want = attention(q[0, :, 0], wk, wv, scale)[0]
+    a = np.abs(q[0, :, 0].astype(np.float64))
+    off = np.where(a >= a.max(-1, keepdims=True) * 2.0 ** (-14 if dtype == 1 else -11), 0.0, 2.0 ** -23 * a.max(-1, keepdims=True))  # [heads, D]
+    score = (off @ np.abs(wk[0].astype(np.float64)).T).max(-1) * scale
+    bound = attention_bound(q[0, :, 0], wk, wv, scale) + 2.1 * score[:, None] * np.abs(wv).max()
+    cache = fb.PagedKvCache(device, 1, 1, D, 44, 44, dtype=fb.I8)
+    cache.append(_T(device, k), _T(device, v))
+    for ctas in (0, 9):
+        cache.set_decode_ctas(ctas)
+        got = cache.decode(_T(device, q, dtype), scale).as_slice()[0, :, 0]
+        assert (np.abs(got - want) <= bound).all(), (ctas, (np.abs(got - want) / bound).max())
